@@ -392,6 +392,136 @@ int rs_qwen_debug_gemm(void* session, int which, int layer, const uint16_t* x, s
 int rs_qwen_project_noalloc(void* session, int which, int layer, const void* x_device, size_t T,
                             float* y_device, size_t y_count, void* stream, char* error, size_t capacity);
 
+/* ---- 4-bit paged KV cache (no reference counterpart) ----
+ *
+ * The attention cache of one layer in 4 bits, on memory the caller owns, for
+ * servers whose contexts do not fit the sessions' bf16 pages. Keys and values
+ * are quantised per (token, KV head) in groups of 64 dims:
+ *   scale = bf16((max - min) / 15), bias = bf16(min),
+ *   n = clamp(rint((x - bias) / scale), 0, 15), value = scale * n + bias
+ * (n = 0 where scale is 0; a group that holds an infinity or NaN reads back as
+ * NaN). A page holds 16 tokens; slot = page * 16 + offset. Of each (page, KV
+ * head) the pool keeps 18 * head_dim bytes (4.5 bits per value; csrc/kv4.h has
+ * the layout), so pool bytes = pages * rs_qwen_kv4_page_bytes.
+ *
+ * Every pointer in the argument structs is device memory of `device`, except
+ * the structs themselves. Calls check their arguments on the host, enqueue on
+ * `stream` (NULL: the legacy default stream) without synchronising and without
+ * allocating, may be captured into a CUDA graph, and leave the calling
+ * thread's current device as it was. Page ids, slots and lengths live on the
+ * device: a kernel skips one that is outside the pool, the table or the
+ * weights' rows (such a key or token counts as absent) and sets bit 2 of
+ * *status, which the caller reads and clears. Calls that share a workspace or
+ * write the same pages must be ordered (one stream, or events). Empty calls
+ * (no tokens, no sequences) succeed and do nothing. */
+#define RS_QWEN_F32 0u
+#define RS_QWEN_F16 1u
+#define RS_QWEN_BF16 2u
+
+typedef struct {
+  int32_t device, q_heads, kv_heads, head_dim; /* head_dim 64, 128 or 256; q_heads / kv_heads 1 to 16 */
+  uint64_t pages;
+  void* pool;       /* 16-byte aligned */
+  uint32_t* status; /* NULL: errors on the device are not reported */
+} rs_qwen_kv4_cache;
+
+/* Rows [token][head][head_dim], strides in elements; head_dim contiguous. */
+typedef struct {
+  const void* data;
+  int64_t token_stride, head_stride;
+} rs_qwen_kv4_rows;
+
+/* Bytes of one page: kv_heads * 18 * head_dim (0 for an unsupported geometry). */
+size_t rs_qwen_kv4_page_bytes(int kv_heads, int head_dim);
+/* Bytes of the workspace rs_qwen_kv4_attention needs for up to n_seq sequences
+ * and `tokens` query tokens (0 for an unsupported geometry). */
+size_t rs_qwen_kv4_workspace_bytes(const rs_qwen_kv4_cache* cache, size_t n_seq, size_t tokens);
+
+/* Per-head RMSNorm of q and k (q_norm / k_norm: head_dim gains, NULL: none),
+ * rotation of the first rope_dims dims (pairs j, j + rope_dims / 2, angle
+ * position * theta^(-2j / rope_dims)), q to q_out, k and v quantised into the
+ * pages. q / k / v share `dtype` and may be strided views of one projection
+ * row. k and v NULL: queries only; q NULL: keys and values only. A negative
+ * slot stores nothing (its q row is still written). The slots of one call must
+ * be distinct. Keys are computed in 64 bits up to the nibble, so the cache does
+ * not depend on the batch around a token. */
+typedef struct {
+  rs_qwen_kv4_rows q, k, v;
+  uint32_t dtype, q_out_dtype;
+  size_t tokens;
+  const float* q_norm;
+  const float* k_norm;
+  const int32_t* positions; /* [tokens], needed when rope_dims > 0 */
+  const int64_t* slots;     /* [tokens] */
+  void* q_out;              /* [tokens][q_heads][head_dim], 16-byte aligned */
+  float epsilon, theta;
+  int32_t rope_dims, reserved;
+} rs_qwen_kv4_append_args;
+int rs_qwen_kv4_append(const rs_qwen_kv4_cache* cache, const rs_qwen_kv4_append_args* args, void* stream, char* error,
+                       size_t capacity);
+
+/* Cached tokens as the values they stand for: k, v [tokens][kv_heads][head_dim]
+ * of `dtype`, 16-byte aligned; a negative slot gives zeros. */
+int rs_qwen_kv4_read(const rs_qwen_kv4_cache* cache, size_t tokens, const int64_t* slots, uint32_t dtype, void* k,
+                     void* v, void* stream, char* error, size_t capacity);
+
+/* out = softmax(scale * q k^T) v over the cached pages, times sigmoid(gate) if
+ * a gate is given. Sequence s owns the query rows cu_seqlens[s] ..
+ * cu_seqlens[s+1] (possibly none; at most max_count, which only steers the
+ * choice of kernel) and the kv_lens[s] keys of the pages block_table[s][...],
+ * its own tokens' keys last and already appended: its query j of n sees the
+ * first kv_lens[s] - n + j + 1 keys. A row that sees none is zero, its lse
+ * -infinity; rows outside [cu_seqlens[0], cu_seqlens[n_seq]) are not written.
+ * q and out are fp16 or bf16 (`dtype`), the gate fp32. lse (or NULL):
+ * [tokens][q_heads], natural logarithm of the sum of exponentials.
+ * weights_out (or NULL): [n_seq][kv_heads][weights_stride], for each key of a
+ * sequence weights_in (NULL: zero) plus the softmax weight it received from all
+ * the call's query rows of its KV head; the newest n keys start from zero.
+ * weights_in may be weights_out. Columns from kv_lens[s] on are not written. */
+typedef struct {
+  rs_qwen_kv4_rows q, gate, out;
+  uint32_t dtype, reserved;
+  size_t n_seq, tokens, max_count;
+  const int32_t* cu_seqlens;  /* [n_seq + 1] */
+  const int32_t* kv_lens;     /* [n_seq] */
+  const int32_t* block_table; /* [n_seq][table_stride] */
+  int64_t table_stride;       /* pages */
+  float scale;                /* 0: 1 / sqrt(head_dim) */
+  float* lse;
+  const float* weights_in;
+  float* weights_out;
+  int64_t weights_stride;
+  void* workspace; /* 16-byte aligned */
+  size_t workspace_bytes;
+} rs_qwen_kv4_attention_args;
+int rs_qwen_kv4_attention(const rs_qwen_kv4_cache* cache, const rs_qwen_kv4_attention_args* args, void* stream,
+                          char* error, size_t capacity);
+
+/* Eviction by accumulated weight, per KV head: of sequence s's kv_lens[s] keys
+ * min(kv_lens[s], keep) stay, in their order: the last `recent` ones and those
+ * of the others with the largest weight (IEEE total order; the lowest index on
+ * ties). They are copied to the pages dst_table[s][...], which must not be
+ * pages of any source sequence. kept [n_seq][kv_heads][keep]: their indices,
+ * then -1; new_lens [n_seq]; weights_out (or NULL)
+ * [n_seq][kv_heads][weights_out_stride]: their weights, then zeros up to keep. */
+typedef struct {
+  size_t n_seq;
+  const int32_t* kv_lens;
+  const int32_t* src_table;
+  int64_t src_stride;
+  const int32_t* dst_table;
+  int64_t dst_stride;
+  const float* weights;
+  int64_t weights_stride;
+  int32_t keep, recent;
+  int32_t* kept;
+  int32_t* new_lens;
+  float* weights_out;
+  int64_t weights_out_stride;
+} rs_qwen_kv4_evict_args;
+int rs_qwen_kv4_evict(const rs_qwen_kv4_cache* cache, const rs_qwen_kv4_evict_args* args, void* stream, char* error,
+                      size_t capacity);
+
 /* Number of floats of a version's reference-layout snapshot
  * (native/qwen_model.inc:268-271 qwen_state_count). */
 size_t rs_qwen_state_count(const rs_qwen_config* config);

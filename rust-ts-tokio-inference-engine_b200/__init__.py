@@ -54,6 +54,47 @@ class StateId(C.Structure):
         return (self.owner, self.slot, self.generation, self.position, self.bytes)
 
 
+class Kv4CacheDesc(C.Structure):
+    """rs_qwen_kv4_cache."""
+
+    _fields_ = [(n, C.c_int32) for n in ("device", "q_heads", "kv_heads", "head_dim")] + [
+        ("pages", C.c_uint64), ("pool", C.c_void_p), ("status", C.c_void_p)]
+
+
+class Kv4Rows(C.Structure):
+    """rs_qwen_kv4_rows."""
+
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class Kv4AppendArgs(C.Structure):
+    """rs_qwen_kv4_append_args."""
+
+    _fields_ = [("q", Kv4Rows), ("k", Kv4Rows), ("v", Kv4Rows), ("dtype", C.c_uint32), ("q_out_dtype", C.c_uint32),
+                ("tokens", C.c_size_t), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("positions", C.c_void_p),
+                ("slots", C.c_void_p), ("q_out", C.c_void_p), ("epsilon", C.c_float), ("theta", C.c_float),
+                ("rope_dims", C.c_int32), ("reserved", C.c_int32)]
+
+
+class Kv4AttentionArgs(C.Structure):
+    """rs_qwen_kv4_attention_args."""
+
+    _fields_ = [("q", Kv4Rows), ("gate", Kv4Rows), ("out", Kv4Rows), ("dtype", C.c_uint32), ("reserved", C.c_uint32),
+                ("n_seq", C.c_size_t), ("tokens", C.c_size_t), ("max_count", C.c_size_t), ("cu_seqlens", C.c_void_p),
+                ("kv_lens", C.c_void_p), ("block_table", C.c_void_p), ("table_stride", C.c_int64), ("scale", C.c_float),
+                ("lse", C.c_void_p), ("weights_in", C.c_void_p), ("weights_out", C.c_void_p),
+                ("weights_stride", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class Kv4EvictArgs(C.Structure):
+    """rs_qwen_kv4_evict_args."""
+
+    _fields_ = [("n_seq", C.c_size_t), ("kv_lens", C.c_void_p), ("src_table", C.c_void_p), ("src_stride", C.c_int64),
+                ("dst_table", C.c_void_p), ("dst_stride", C.c_int64), ("weights", C.c_void_p),
+                ("weights_stride", C.c_int64), ("keep", C.c_int32), ("recent", C.c_int32), ("kept", C.c_void_p),
+                ("new_lens", C.c_void_p), ("weights_out", C.c_void_p), ("weights_out_stride", C.c_int64)]
+
+
 assert C.sizeof(RsQwenConfig) == 132 and C.sizeof(StateId) == 40
 
 _P, _SZ, _U32P, _F32P, _I32P = C.c_void_p, C.c_size_t, C.POINTER(C.c_uint32), C.POINTER(C.c_float), C.POINTER(C.c_int32)
@@ -118,6 +159,12 @@ SIGNATURES = {
                                      C.POINTER(C.c_double), _ERR, _SZ]),
     "rs_qwen_project_noalloc": (C.c_int, [_P, C.c_int, C.c_int, C.c_void_p, _SZ, C.c_void_p, _SZ, C.c_void_p,
                                           _ERR, _SZ]),
+    "rs_qwen_kv4_page_bytes": (_SZ, [C.c_int, C.c_int]),
+    "rs_qwen_kv4_workspace_bytes": (_SZ, [C.POINTER(Kv4CacheDesc), _SZ, _SZ]),
+    "rs_qwen_kv4_append": (C.c_int, [C.POINTER(Kv4CacheDesc), C.POINTER(Kv4AppendArgs), _P, _ERR, _SZ]),
+    "rs_qwen_kv4_read": (C.c_int, [C.POINTER(Kv4CacheDesc), _SZ, _P, C.c_uint32, _P, _P, _P, _ERR, _SZ]),
+    "rs_qwen_kv4_attention": (C.c_int, [C.POINTER(Kv4CacheDesc), C.POINTER(Kv4AttentionArgs), _P, _ERR, _SZ]),
+    "rs_qwen_kv4_evict": (C.c_int, [C.POINTER(Kv4CacheDesc), C.POINTER(Kv4EvictArgs), _P, _ERR, _SZ]),
 }
 
 _lib = None
@@ -486,3 +533,166 @@ class DeviceSession:
         out = np.zeros((self.cfg.layers, tokens, self.cfg.top), np.int32)
         _call("rs_qwen_device_debug_routing", self.h, _ptr(out, C.c_int32), out.size)
         return out
+
+
+# ---- 4-bit paged KV cache ----
+
+KV4_PAGE = 16  # tokens per page
+_KV4_TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+
+
+def kv4_page_bytes(kv_heads: int, head_dim: int) -> int:
+    """Pool bytes of one 16-token page (rs_qwen_kv4_page_bytes)."""
+    n = load().rs_qwen_kv4_page_bytes(kv_heads, head_dim)
+    if not n:
+        raise NativeError("kv4: head_dim must be 64, 128 or 256 and kv_heads 1 to 1024")
+    return n
+
+
+class Kv4Cache:
+    """4-bit paged KV cache of one attention layer (rs_qwen_kv4_*) on CUDA tensors.
+
+    `pool` is a contiguous uint8 tensor holding whole pages (kv4_page_bytes each);
+    it stays the caller's. Every other argument is a tensor on the pool's device.
+    Calls enqueue on `stream` (a torch stream or raw handle; default: the current
+    stream of that device) and do not synchronise; a tensor that belongs to
+    another stream must be kept alive and ordered by the caller, as for any
+    kernel. `status`, a one-element int32 tensor, receives bit 2 when a kernel
+    met a page id, slot or length out of range (see check())."""
+
+    def __init__(self, pool, q_heads: int, kv_heads: int, head_dim: int, status=None):
+        page = kv4_page_bytes(kv_heads, head_dim)
+        if str(pool.dtype) != "torch.uint8" or not pool.is_contiguous() or not pool.is_cuda:
+            raise ValueError("kv4: the pool is a contiguous uint8 CUDA tensor")
+        if pool.numel() < page or pool.numel() % page:
+            raise ValueError(f"kv4: the pool holds whole pages of {page} bytes")
+        if status is not None and (str(status.dtype) != "torch.int32" or status.numel() != 1 or
+                                   status.device != pool.device):
+            raise ValueError("kv4: status is one int32 on the pool's device")
+        self.pool, self.status, self.device = pool, status, pool.device
+        self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
+        self.pages = pool.numel() // page
+        self.desc = Kv4CacheDesc(pool.device.index, q_heads, kv_heads, head_dim, self.pages, pool.data_ptr(),
+                                 None if status is None else status.data_ptr())
+        self._ref = C.byref(self.desc)
+        if not load().rs_qwen_kv4_workspace_bytes(self._ref, 1, 1):
+            raise NativeError("kv4: q_heads must be 1 to 16 times kv_heads")
+
+    def _stream(self, stream):
+        if stream is None:
+            import torch
+            return torch.cuda.current_stream(self.device).cuda_stream
+        return getattr(stream, "cuda_stream", stream)
+
+    def _rows(self, x, name, tokens, heads, dtype=None):
+        if x is None:
+            return Kv4Rows()
+        if x.device != self.device or x.dim() != 3 or tuple(x.shape) != (tokens, heads, self.head_dim):
+            raise ValueError(f"kv4: {name} must be [{tokens}, {heads}, {self.head_dim}] on {self.device}")
+        if dtype is not None and x.dtype != dtype:
+            raise ValueError(f"kv4: {name} must be {dtype}")
+        s = x.stride()
+        if s[2] != 1 and x.numel():
+            raise ValueError(f"kv4: the last dimension of {name} must be contiguous")
+        return Kv4Rows(x.data_ptr(), s[0], s[1])
+
+    def _array(self, x, name, dtype, shape=None, optional=False):
+        """Pointer of a contiguous array."""
+        if x is None:
+            if optional:
+                return None
+            raise ValueError(f"kv4: {name} is missing")
+        if x.device != self.device or str(x.dtype) != dtype or not x.is_contiguous():
+            raise ValueError(f"kv4: {name} must be a contiguous {dtype} tensor on {self.device}")
+        if shape is not None and tuple(x.shape) != shape:
+            raise ValueError(f"kv4: {name} must be of shape {list(shape)}")
+        return x.data_ptr()
+
+    def _type(self, x, name):
+        code = _KV4_TYPES.get(str(x.dtype))
+        if code is None:
+            raise ValueError(f"kv4: {name} must be float32, float16 or bfloat16")
+        return code
+
+    def workspace_bytes(self, n_seq: int, tokens: int) -> int:
+        """Workspace of attention() for up to this many sequences and query tokens."""
+        return load().rs_qwen_kv4_workspace_bytes(self._ref, n_seq, tokens)
+
+    def append(self, q, k, v, positions, slots, q_out, q_norm=None, k_norm=None, epsilon: float = 1e-6,
+               theta: float = 1e7, rope_dims: int = 0, stream=None):
+        """Norm, rotation and 4-bit write of new tokens (rs_qwen_kv4_append). q [T, q_heads, D], k and v
+        [T, kv_heads, D] of one dtype, any token / head strides; q (with q_out) or k and v may be None."""
+        x = q if q is not None else k
+        if x is None or (k is None) != (v is None) or (q is None) != (q_out is None):
+            raise ValueError("kv4: append takes q with q_out, k with v, or all four")
+        T = x.shape[0]
+        one = "torch.float32"
+        args = Kv4AppendArgs(
+            self._rows(q, "q", T, self.q_heads, x.dtype), self._rows(k, "k", T, self.kv_heads, x.dtype),
+            self._rows(v, "v", T, self.kv_heads, x.dtype), self._type(x, "q"),
+            0 if q_out is None else self._type(q_out, "q_out"), T,
+            self._array(q_norm, "q_norm", one, (self.head_dim,), True),
+            self._array(k_norm, "k_norm", one, (self.head_dim,), True),
+            self._array(positions, "positions", "torch.int32", (T,), rope_dims == 0),
+            self._array(slots, "slots", "torch.int64", (T,), k is None),
+            None if q_out is None else self._array(q_out, "q_out", str(q_out.dtype), (T, self.q_heads, self.head_dim)),
+            epsilon, theta, rope_dims, 0)
+        _call("rs_qwen_kv4_append", self._ref, C.byref(args), self._stream(stream))
+
+    def read(self, slots, k, v, stream=None):
+        """Cached tokens back as values (rs_qwen_kv4_read): k, v [len(slots), kv_heads, D]."""
+        shape = (slots.shape[0], self.kv_heads, self.head_dim)
+        _call("rs_qwen_kv4_read", self._ref, shape[0], self._array(slots, "slots", "torch.int64", shape[:1]),
+              self._type(k, "k"), self._array(k, "k", str(k.dtype), shape), self._array(v, "v", str(k.dtype), shape),
+              self._stream(stream))
+
+    def attention(self, q, cu_seqlens, kv_lens, block_table, out, workspace, max_count: int, gate=None, lse=None,
+                  weights_in=None, weights_out=None, scale: float = 0.0, stream=None):
+        """Ragged causal attention over the pages (rs_qwen_kv4_attention). block_table: int32 [n_seq, pages];
+        weights_in / weights_out: float32 [n_seq, kv_heads, columns]; workspace: uint8, workspace_bytes()."""
+        T, n, dim = q.shape[0], kv_lens.shape[0], q.dim()
+        if dim != 3 or block_table.dim() != 2:
+            raise ValueError("kv4: q must be [T, q_heads, head_dim] and block_table [n_seq, pages]")
+        if gate is not None and str(gate.dtype) != "torch.float32":
+            raise ValueError("kv4: the gate must be float32")
+        one, whole = "torch.float32", "torch.int32"
+        columns = 0
+        if weights_out is not None:
+            columns = weights_out.shape[-1]
+        elif weights_in is not None:
+            raise ValueError("kv4: weights_in needs weights_out")
+        wshape = (n, self.kv_heads, columns)
+        args = Kv4AttentionArgs(
+            self._rows(q, "q", T, self.q_heads), self._rows(gate, "gate", T, self.q_heads),
+            self._rows(out, "out", T, self.q_heads, q.dtype), self._type(q, "q"), 0, n, T, max_count,
+            self._array(cu_seqlens, "cu_seqlens", whole, (n + 1,)), self._array(kv_lens, "kv_lens", whole, (n,)),
+            self._array(block_table, "block_table", whole, (n, block_table.shape[1])), block_table.shape[1], scale,
+            self._array(lse, "lse", one, (T, self.q_heads), True),
+            self._array(weights_in, "weights_in", one, wshape, True),
+            self._array(weights_out, "weights_out", one, wshape, True), columns,
+            self._array(workspace, "workspace", "torch.uint8"), workspace.numel())
+        _call("rs_qwen_kv4_attention", self._ref, C.byref(args), self._stream(stream))
+
+    def evict(self, kv_lens, src_table, dst_table, weights, keep: int, recent: int, kept, new_lens, weights_out=None,
+              stream=None):
+        """Keeps the most attended keys of every sequence and KV head (rs_qwen_kv4_evict); the kept keys move to
+        the pages of dst_table."""
+        n, one, whole = kv_lens.shape[0], "torch.float32", "torch.int32"
+        args = Kv4EvictArgs(
+            n, self._array(kv_lens, "kv_lens", whole, (n,)),
+            self._array(src_table, "src_table", whole, (n, src_table.shape[1])), src_table.shape[1],
+            self._array(dst_table, "dst_table", whole, (n, dst_table.shape[1])), dst_table.shape[1],
+            self._array(weights, "weights", one, (n, self.kv_heads, weights.shape[-1])), weights.shape[-1], keep, recent,
+            self._array(kept, "kept", whole, (n, self.kv_heads, keep)), self._array(new_lens, "new_lens", whole, (n,)),
+            self._array(weights_out, "weights_out", one,
+                        None if weights_out is None else (n, self.kv_heads, weights_out.shape[-1]), True),
+            0 if weights_out is None else weights_out.shape[-1])
+        _call("rs_qwen_kv4_evict", self._ref, C.byref(args), self._stream(stream))
+
+    def check(self):
+        """Reads and clears the status word (synchronises); raises if a kernel met an index out of range."""
+        if self.status is not None:
+            bits = int(self.status.item())
+            if bits:
+                self.status.zero_()
+                raise NativeError(f"kv4: device error flag {bits}")

@@ -467,8 +467,8 @@ int rs_qwen_kv4_read(const rs_qwen_kv4_cache* cache, size_t tokens, const int64_
 
 /* out = softmax(scale * q k^T) v over the cached pages, times sigmoid(gate) if
  * a gate is given. Sequence s owns the query rows cu_seqlens[s] ..
- * cu_seqlens[s+1] (possibly none; at most max_count, which only steers the
- * choice of kernel) and the kv_lens[s] keys of the pages block_table[s][...],
+ * cu_seqlens[s+1] (possibly none; more than max_count set the status bit and
+ * are not computed) and the kv_lens[s] keys of the pages block_table[s][...],
  * its own tokens' keys last and already appended: its query j of n sees the
  * first kv_lens[s] - n + j + 1 keys. A row that sees none is zero, its lse
  * -infinity; rows outside [cu_seqlens[0], cu_seqlens[n_seq]) are not written.

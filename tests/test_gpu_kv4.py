@@ -304,6 +304,28 @@ def test_nan_in_the_cache_reaches_only_its_own_rows(pkg):
     assert torch.isnan(out[2:4]).all()
 
 
+def test_nan_value_reaches_only_the_rows_that_see_it(pkg):
+    seqs = Sequences(pkg, [20], (4, 2, 64), seed=26)
+    q, cu, host = seqs.queries([4], torch.float16)
+    good, _, _ = attend(pkg, seqs, q, cu, [4])
+    slot = seqs.slots(0, 18, 19)
+    k_old, _ = read(seqs.cache, slot)
+    seqs.cache.append(None, k_old, torch.full((1, 2, 64), math.inf, device="cuda"), None, slot, None)
+    out, _, _ = attend(pkg, seqs, q, cu, [4])
+    assert torch.equal(out[:2], good[:2]) and torch.isnan(out[2:]).all()
+
+
+def test_more_rows_than_max_count_are_reported(pkg):
+    seqs = Sequences(pkg, [20, 20], (4, 2, 64), seed=27)
+    q, cu, host = seqs.queries([4, 2], torch.float16)
+    want, _, _ = attend(pkg, seqs, q, cu, [4, 2])
+    seqs.cache.check()
+    out, _, _ = attend(pkg, seqs, q, cu, [2, 2])  # claims two rows at most
+    assert torch.equal(out[4:], want[4:]) and (out[:4] == 77).all()
+    with pytest.raises(pkg.NativeError, match="flag 2"):
+        seqs.cache.check()
+
+
 def test_strided_queries_and_outputs(pkg):
     heads = (8, 2, 128)
     seqs = Sequences(pkg, [50, 7, 200], heads, seed=15)
@@ -441,9 +463,9 @@ def test_captured_and_replayed(pkg):
         with torch.cuda.graph(graph, stream=side):
             seqs.cache.append(q_in, k, v, pos, slots, q, rope_dims=64)
             seqs.cache.attention(q, cu, seqs.kv_lens, seqs.table, out, ws, 1)
-        graphs.append((seqs, q_in, k, v, pos, slots, q, out, graph))
+        graphs.append((seqs, q_in, k, v, pos, slots, q, out, (cu, ws), graph))  # a graph's buffers live as long as it
     for step in range(3):
-        for seqs, q_in, k, v, pos, slots, q, out, graph in graphs:
+        for seqs, q_in, k, v, pos, slots, q, out, _, graph in graphs:
             for x in (q_in, k, v):
                 x.normal_()
             pos.copy_(seqs.kv_lens)
@@ -460,7 +482,7 @@ def test_captured_and_replayed(pkg):
         for g in graphs:
             g[-1].replay()
         torch.cuda.synchronize()
-        for seqs, q_in, k, v, pos, slots, q, out, graph in graphs:
+        for seqs, q_in, k, v, pos, slots, q, out, _, graph in graphs:
             check_attention(seqs, q, [0, 1, 2], out)
             seqs.cache.check()
 

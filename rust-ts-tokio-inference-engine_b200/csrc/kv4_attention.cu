@@ -1,20 +1,22 @@
 // Attention over the 4-bit paged KV cache.
 //
 // kv4_decode_kernel: the (sequence, KV head, tile of 8 query rows) units of a
-// call are laid end to end, measured in the pages each has to read, and cut
+// call are laid end to end, measured in the page pairs each has to read, and cut
 // into equal ranges, one per CTA; a unit that spans CTAs leaves partial results
 // that kv4_merge_kernel joins. The lengths live on the device, so every CTA
 // finds its range itself from a prefix sum over the sequences.
 //
-// The pages of a range are dealt to the CTA's warps through private
-// shared-memory rings; in one more warp each lane owns a ring slot and keeps it
-// filled, one bulk copy per (page, KV head) block, across unit borders. A warp
-// works on 16 keys x 8 query rows:
+// The pairs of a range are dealt to the CTA's warps, which stream them through
+// private shared-memory rings, one bulk copy per (page, KV head) block; a ring
+// runs on across unit borders. A warp works on 2 x 16 keys x 8 query rows:
 //   S^T = K Q^T. An fp16 subnormal with the bits 0000 0000 0000 nnnn is n 2^-24
 //   and one with nnnn 0000 is n 2^-20, exactly, so the masks 0x000F000F and
 //   0x00F000F0 turn a word of nibbles into MMA operands with no conversion; the
 //   factor 2^4 between the two is taken out of Q. Scale and bias of a group of
 //   64 dims enter afterwards in 32 bits: s = scale (q . n) + bias (sum of q).
+//   The stored pairs (scale, bias) are themselves a bf16 operand: against
+//   (0, sum of q), the sums split into three bf16 terms, two MMAs give the
+//   bias part of all 16 keys.
 //   Q is fp16, each row scaled by a power of two, so fp16 and bf16 queries are
 //   exact (bf16 has fewer mantissa bits and the row keeps its range).
 //   O^T += V^T P^T. The nibbles of two keys are interleaved into k pairs and
@@ -39,13 +41,14 @@ extern std::atomic<uint64_t> g_kernel_launches;
 
 namespace {
 
-constexpr int kWarps = 4;   // that compute; one more fetches
-constexpr int kStages = 4;  // pages of a warp's ring
-constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kWarps = 4;
+constexpr int kStages = 2;  // page pairs of a warp's ring
+constexpr int kThreads = kWarps * 32;
 constexpr int kCtasPerSm = 2;
 constexpr int kRowsPerTile = 8;
-constexpr int kMinPages = 8;  // fewest pages of a CTA's range
-static_assert(kWarps * kStages <= 32, "one fetching lane per ring slot");
+constexpr int kMinPairs = 8;   // fewest page pairs of a CTA's range
+constexpr int kUnitPairs = 3;  // what a unit costs beside its pages, in page pairs
+constexpr int kGroupsMax = 512;  // entries of the prefix table that finds a page's sequence
 constexpr float kLazy = 8.f;    // log2 of how far a logit may exceed the running maximum
 constexpr long long kWaitCycles = 2000000000ll;
 
@@ -70,17 +73,6 @@ __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {  // does not wait
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32_t* status) {
   if (mbar_try(bar, parity)) return true;
   const long long t0 = clock64();
@@ -100,20 +92,48 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// d = a b from zero accumulators (no registers to clear)
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
+}
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
+  if constexpr (N == 4) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
+  else if constexpr (N == 2) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+  else w[0] = *reinterpret_cast<const uint32_t*>(p);
 }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -156,9 +176,15 @@ __device__ __forceinline__ int tile_pages(const Seq& q, int r, int G) {
   const int token = min(q.count - 1, ((r + 1) * kRowsPerTile - 1) / G);
   return max(0, q.len - q.count + token + 1 + kPageTokens - 1) / kPageTokens;
 }
-__device__ __forceinline__ int64_t seq_pages(const Seq& q, int G) {  // of one KV head
+// Length of a unit: its page pairs behind kUnitPairs places that hold none, so
+// that ranges of equal length take equal time whatever the units' sizes.
+__device__ __forceinline__ int unit_length(const Seq& q, int r, int G) {
+  const int pages = tile_pages(q, r, G);
+  return pages ? (pages + 1) / 2 + kUnitPairs : 0;
+}
+__device__ __forceinline__ int64_t seq_length(const Seq& q, int G) {  // of one KV head
   int64_t n = 0;
-  for (int r = 0; r < q.tiles; ++r) n += tile_pages(q, r, G);
+  for (int r = 0; r < q.tiles; ++r) n += unit_length(q, r, G);
   return n;
 }
 
@@ -183,13 +209,18 @@ __host__ __device__ inline Workspace carve(void* base, int n_seq, int ctas) {
   return w;
 }
 
-// Writes 8 dims of one output row: y / l, gated.
-template <class T>
-__device__ __forceinline__ void write_dims(const Kv4AttentionArgs& a, int token, int head, int dim, float (&y)[8], bool vec) {
-  if (a.gate.data) {
-    const float* g = static_cast<const float*>(a.gate.data) + token * a.gate.token_stride + head * a.gate.head_stride + dim;
+// Writes 8 dims of one output row, gated.
+__device__ __forceinline__ void load_gate(const Kv4AttentionArgs& a, int token, int head, int dim, float (&g)[8]) {
+  const float* p = static_cast<const float*>(a.gate.data) + token * a.gate.token_stride + head * a.gate.head_stride + dim;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] *= sigmoidf_(g[i]);
+  for (int i = 0; i < 8; ++i) g[i] = p[i];
+}
+template <class T>
+__device__ __forceinline__ void write_dims(const Kv4AttentionArgs& a, int token, int head, int dim, float (&y)[8],
+                                           const float (&gate)[8], bool vec) {
+  if (a.gate.data) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] *= sigmoidf_(gate[i]);
   }
   T* out = static_cast<T*>(a.out) + token * a.out_token_stride + head * a.out_head_stride + dim;
   alignas(16) T v[8];
@@ -205,17 +236,97 @@ __device__ __forceinline__ void write_dims(const Kv4AttentionArgs& a, int token,
 
 template <int D>
 struct Smem {
-  alignas(128) uint8_t ring[kWarps][kStages][Kv4Layout<D>::kBlock];
-  alignas(16) float o[kRowsPerTile][D];
+  alignas(128) uint8_t ring[kWarps][kStages][2][Kv4Layout<D>::kBlock];
+  alignas(16) float o[2][kRowsPerTile][D];
+  alignas(16) uint32_t q[Kv4Layout<D>::kLaneWords][32][4];  // B fragments of the tile's rows
+  uint32_t q_sum[3][kRowsPerTile][4];  // sums over the groups as bf16 terms, above a zero
+  float q_back[kRowsPerTile];
+  int q_seen[kRowsPerTile];
   float ml[kWarps][kRowsPerTile][2];
-  int64_t scan[kWarps + 1];
-  int64_t start_offset;
-  int start_seq;
-  int absent[kWarps][kStages];  // the slot's page is outside the pool
-  uint64_t full[kWarps][kStages], empty[kWarps][kStages];
+  int64_t scan[kWarps];
+  int64_t offsets[kGroupsMax + 1];  // first place of each group of sequences
+  alignas(16) uint64_t blocks[kWarps][64][2];  // blocks of a warp's next places, two windows of 32; 0: none
+  int start;                        // the group that holds the range's first place
+  uint64_t full[kWarps][kStages];
 };
 
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
+// The query rows of a tile as B fragments (lane = 4 row + t, register j of word
+// i: dims 2 j, 2 j + 1 of the word's eight), 16 threads per row. A row is
+// scaled by a power of two so that its largest value lies in [2^13, 2^14):
+// fp16 and bf16 queries stay exact; the pairs that meet nibbles carrying 2^4
+// are lowered by as much. Beside them: the factor that brings (q . n) 2^-24
+// back to a logit in base 2, the row's sums over the groups in base 2, and how
+// many keys it sees. A row with a value that is not finite gets NaN sums, so
+// its logits are all NaN.
+template <int D, class T>
+__device__ __forceinline__ void load_tile(const Kv4AttentionArgs& a, const Seq& seq, int head0, int r, int G, bool vec,
+                                          int tid, uint32_t (*frag)[32][4], uint32_t (*sums)[kRowsPerTile][4], float* back, int* seen) {
+  constexpr int kPer = D / 128 > 0 ? D / 128 : 1;  // words of a thread
+  const int rr = tid / 16, j = tid % 16, row = r * kRowsPerTile + rr, token = row / G;
+  const bool real = token < seq.count;
+  const T* src = static_cast<const T*>(a.q.data) + (seq.first + token) * a.q.token_stride + (head0 + row % G) * a.q.head_stride;
+  float x[kPer][8], most = 0.f, sum[kPer];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int w = j + 16 * k;
+    alignas(16) T raw[8] = {};
+    if (real && w < D / 8) {
+      if (vec) {
+        *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(src + 8 * w);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) raw[e] = src[8 * w + e];
+      }
+    }
+    sum[k] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[k][e] = kv4_to_float(raw[e]);
+      sum[k] += x[k][e];
+      // the largest magnitude; a NaN's bits are above every number's
+      most = __uint_as_float(max(__float_as_uint(most), __float_as_uint(x[k][e]) & 0x7FFFFFFFu));
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) most = __uint_as_float(max(__float_as_uint(most), __shfl_xor_sync(0xffffffffu, __float_as_uint(most), o)));
+  const bool fine = __float_as_uint(most) < 0x7F800000u;
+  const int e = most > 0.f && fine ? int(__float_as_uint(most) >> 23) - 126 : 0;  // |row| < 2^e
+  const float up = pow2i((14 - e) / 2), up2 = fine ? pow2i(14 - e - (14 - e) / 2) : 0.f;
+  const float factor = a.scale * 1.4426950408889634f;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int w = j + 16 * k;
+    if (w < D / 8) {
+      uint32_t v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float lift = (i & 1 ? 0.0625f : 1.f) * up2;
+        v[i] = fine ? pack_f16(x[k][2 * i] * up * lift, x[k][2 * i + 1] * up * lift) : 0u;
+      }
+      *reinterpret_cast<uint4*>(frag[2 * (w / 8) + w % 8 / 4][4 * rr + w % 4]) = make_uint4(v[0], v[1], v[2], v[3]);
+      if (w % 8 == 0) {
+        const float total = fine ? sum[k] * factor : NAN;
+        float rest = total;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const uint32_t top = uint32_t(float_to_bf16_bits(rest)) << 16;
+          sums[i][rr][w / 8] = top;
+          rest -= __uint_as_float(top);
+        }
+      }
+    }
+  }
+  if (j >= D / 64 && j < 4) {  // groups this head_dim does not have
+#pragma unroll
+    for (int i = 0; i < 3; ++i) sums[i][rr][j] = 0u;
+  }
+  if (j == 0) {
+    back[rr] = factor * pow2i((e + 10) / 2) * pow2i(e + 10 - (e + 10) / 2);
+    seen[rr] = real ? seq.len - seq.count + token + 1 : INT_MAX;  // rows past the last are not written
+  }
+}
 
 // Position in the laid-out units.
 struct Cursor {
@@ -224,7 +335,7 @@ struct Cursor {
 };
 
 template <int D, class T>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4AttentionArgs a, bool out_vec) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4AttentionArgs a, bool q_vec, bool out_vec) {
   pdl_trigger();
   pdl_wait();
   using L = Kv4Layout<D>;
@@ -234,67 +345,76 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, tq = lane & 3;
   const int Hkv = a.cache.Hkv, G = a.cache.Hq / Hkv;
   const Workspace ws = carve(a.workspace, a.n_seq, gridDim.x);
-  if (tid < kWarps * kStages) {
-    mbar_init(&sm.full[0][0] + tid, 1);
-    mbar_init(&sm.empty[0][0] + tid, 1);
-  }
+  if (tid < kWarps * kStages) mbar_init(&sm.full[0][0] + tid, 1);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 
-  // total pages, then the sequence in which this CTA's range starts
+  // page offsets of the sequences, in groups of `per` when there are many
+  const int per = (a.n_seq + kGroupsMax - 1) / kGroupsMax, groups = (a.n_seq + per - 1) / per;
   int64_t total = 0;
-  {
-    int64_t mine = 0;
-    for (int s = tid; s < a.n_seq; s += blockDim.x)
-      mine += seq_pages(load_seq(a, s, G, blockIdx.x == 0), G) * Hkv;
+  for (int g0 = 0; g0 < groups; g0 += kThreads) {
+    const int gi = g0 + tid;
+    int64_t n = 0;
+    for (int s = gi * per; s < min(a.n_seq, (gi + 1) * per); ++s)
+      n += seq_length(load_seq(a, s, G, blockIdx.x == 0), G) * Hkv;
+    int64_t x = n;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) sm.scan[warp] = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) sm.scan[warp] = x;
     __syncthreads();
+    int64_t before = total;
 #pragma unroll
-    for (int w = 0; w <= kWarps; ++w) total += sm.scan[w];
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += sm.scan[w];
+      total += sm.scan[w];
+    }
+    if (gi < groups) sm.offsets[gi] = before + x - n;
     __syncthreads();
   }
-  const int64_t range = max(int64_t(kMinPages), (total + gridDim.x - 1) / gridDim.x);
+  if (tid == 0) sm.offsets[groups] = total;
+  __syncthreads();
+  const int64_t range = max(int64_t(kMinPairs), (total + gridDim.x - 1) / gridDim.x);
   const int64_t begin = blockIdx.x * range, end = min(total, begin + range);
-  if (blockIdx.x == 0 && tid == 0) *ws.range = range;
-  if (begin < end || blockIdx.x == 0) {
-    int64_t base = 0;
-    for (int s0 = 0; s0 < a.n_seq; s0 += blockDim.x) {
-      const int s = s0 + tid;
-      const int64_t n = s < a.n_seq ? seq_pages(load_seq(a, s, G, false), G) * Hkv : 0;
-      int64_t x = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+  if (blockIdx.x == 0) {  // for the merge
+    for (int gi = tid; gi < groups; gi += kThreads) {
+      int64_t off = sm.offsets[gi];
+      for (int s = gi * per; s < min(a.n_seq, (gi + 1) * per); ++s) {
+        ws.offsets[s] = off;
+        off += seq_length(load_seq(a, s, G, false), G) * Hkv;
       }
-      if (lane == 31) sm.scan[warp] = x;
-      __syncthreads();
-      int64_t before = base, sum = 0;
-#pragma unroll
-      for (int w = 0; w <= kWarps; ++w) {
-        if (w < warp) before += sm.scan[w];
-        sum += sm.scan[w];
-      }
-      const int64_t off = before + x - n;
-      if (blockIdx.x == 0) {
-        if (s < a.n_seq) ws.offsets[s] = off;
-        if (s == a.n_seq - 1) ws.offsets[a.n_seq] = off + n;
-      }
-      if (n && begin >= off && begin < off + n) {
-        sm.start_seq = s;
-        sm.start_offset = off;
-      }
-      base += sum;
-      __syncthreads();
+    }
+    if (tid == 0) {
+      ws.offsets[a.n_seq] = total;
+      *ws.range = range;
     }
   }
   if (begin >= end) return;
 
-  // cursor at the unit that holds `begin`
-  auto advance = [&](Cursor& c, Seq& q, int& pages) {  // to the next unit with pages
+  // the unit that holds place p, in or behind group gi
+  auto locate = [&](int64_t p, int gi, Cursor& c, Seq& q) {
+    c.s = gi * per;
+    c.at = sm.offsets[gi];
+    int64_t one;
+    for (;;) {
+      q = load_seq(a, c.s, G, false);
+      one = seq_length(q, G);
+      if (c.at + one * Hkv > p) break;
+      c.at += one * Hkv;
+      ++c.s;
+    }
+    c.g = 0;
+    while (c.at + one <= p) {
+      c.at += one;
+      ++c.g;
+    }
+    c.r = 0;
+    while (c.at + unit_length(q, c.r, G) <= p) c.at += unit_length(q, c.r++, G);
+  };
+  auto advance = [&](Cursor& c, Seq& q, int& length) {  // to the next unit that has pages
     do {
-      c.at += pages;
+      c.at += length;
       if (++c.r >= q.tiles) {
         c.r = 0;
         if (++c.g >= Hkv) {
@@ -303,117 +423,90 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
           while (q.tiles == 0);
         }
       }
-      pages = tile_pages(q, c.r, G);
-    } while (pages == 0);
+      length = unit_length(q, c.r, G);
+    } while (length == 0);
   };
-  Cursor u{sm.start_seq, 0, 0, sm.start_offset};
-  Seq seq = load_seq(a, u.s, G, false);
-  int pages = tile_pages(seq, 0, G);
-  while (pages == 0 || u.at + pages <= begin) advance(u, seq, pages);
+  for (int gi = tid; gi < groups; gi += kThreads)
+    if (sm.offsets[gi] <= begin && begin < sm.offsets[gi + 1]) sm.start = gi;
+  __syncthreads();
+  Cursor u;
+  Seq seq;
+  locate(begin, sm.start, u, seq);
+  int length = unit_length(seq, u.r, G);
 
-  if (warp == kWarps) {
-    // lane = (warp, slot): its pages are begin + warp + kWarps (slot + kStages n)
-    if (lane >= kWarps * kStages) return;
-    const int w = lane / kStages, slot = lane % kStages;
-    int64_t p = begin + w + int64_t(kWarps) * slot;
-    int64_t block = -1;
-    auto look_up = [&] {
-      while (u.at + pages <= p) advance(u, seq, pages);
-      const int64_t page = a.table[u.s * a.table_stride + (p - u.at)];
-      const bool ok = page >= 0 && uint64_t(page) < a.cache.pages;
-      if (!ok) kv4_flag(a.cache.status, kErrBounds);
-      block = ok ? page * Hkv + u.g : -1;
-    };
-    if (p < end) look_up();
-    uint32_t n = 0;  // pages this lane has fetched
-    long long t0 = clock64();
-    while (p < end) {
-      if (n == 0 || mbar_test(&sm.empty[w][slot], (n - 1) & 1u)) {
-        sm.absent[w][slot] = block < 0;
-        if (block < 0) {
-          mbar_arrive(&sm.full[w][slot]);
-        } else {
-          mbar_expect_tx(&sm.full[w][slot], L::kBlock);
-          bulk_load(sm.ring[w][slot], a.cache.pool + uint64_t(block) * L::kBlock, L::kBlock, &sm.full[w][slot]);
-        }
-        ++n;
-        p += kWarps * kStages;
-        if (p < end) look_up();
-        t0 = clock64();
-      } else if (clock64() - t0 > 2 * kWaitCycles) {
-        kv4_flag(a.cache.status, kErrTimeout);
-        break;
-      } else {
-        __nanosleep(40);
+  // the warp's places are begin + warp + kWarps i; window w holds i = 32 w .. 32 w + 31
+  const int n_mine = int((end - begin - warp + kWarps - 1) / kWarps);
+  auto look_up = [&](int i) {
+    if (i >= n_mine) return;
+    const int64_t p = begin + warp + int64_t(kWarps) * i;
+    Cursor c = u;
+    Seq q = seq;
+    if (p >= u.at + length) {
+      int lo = sm.start, hi = groups;  // the last group that starts at or before p
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (sm.offsets[mid] <= p) lo = mid;
+        else hi = mid;
       }
+      locate(p, lo, c, q);
     }
-    // every copy has landed before the CTA may leave
-    if (n) mbar_wait(&sm.full[w][slot], (n - 1) & 1u, a.cache.status);
-    return;
-  }
+    const int64_t at = (p - c.at - kUnitPairs) * 2;
+    const int pages = tile_pages(q, c.r, G);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint64_t block = 0;
+      if (at >= 0 && at + h < pages) {
+        const int64_t page = a.table[c.s * a.table_stride + at + h];
+        if (page >= 0 && uint64_t(page) < a.cache.pages) block = reinterpret_cast<uint64_t>(a.cache.block(uint64_t(page), c.g));
+        else kv4_flag(a.cache.status, kErrBounds);
+      }
+      sm.blocks[warp][i & 63][h] = block;
+    }
+  };
+  auto issue = [&](int i, int stage) {  // lane 0
+    if (i >= n_mine) return;
+    const ulonglong2 from = *reinterpret_cast<const ulonglong2*>(sm.blocks[warp][i & 63]);
+    uint64_t* bar = &sm.full[warp][stage];
+    if (!(from.x | from.y)) {
+      mbar_arrive(bar);
+      return;
+    }
+    mbar_expect_tx(bar, (from.x ? L::kBlock : 0) + (from.y ? L::kBlock : 0));
+    if (from.x) bulk_load(sm.ring[warp][stage][0], reinterpret_cast<const void*>(from.x), L::kBlock, bar);
+    if (from.y) bulk_load(sm.ring[warp][stage][1], reinterpret_cast<const void*>(from.y), L::kBlock, bar);
+  };
+  look_up(lane);
+  __syncwarp();
+  if (lane == 0)
+    for (int i = 0; i < kStages; ++i) issue(i, i);
 
   bool alive = true;  // false after a wait ran out
-  int done = 0;       // pages this warp has finished
-  {
-    while (true) {  // units of the range
-      const int64_t u_begin = max(u.at, begin), u_end = min(u.at + pages, end);
-      // query rows of the tile: B fragments (row gr), sums and factors (rows 2 tq, 2 tq + 1)
-      static_assert(sizeof(T) == 2, "query type");
+  int place = warp;   // the warp's next place, from `begin`
+  while (true) {  // units of the range
+    const int64_t u_begin = max(u.at, begin), u_end = min(u.at + length, end);
+    const bool whole = u.at >= begin && u.at + length <= end;
+    const int slot = u_begin == begin ? 0 : 1;
+    if (u_end <= u.at + kUnitPairs) {  // none of its pages lies in the range
+      for (int e = tid; e < kRowsPerTile; e += kThreads) {
+        float* ml = ws.ml + ((size_t(blockIdx.x) * 2 + slot) * kRowsPerTile + e) * 2;
+        ml[0] = -FLT_MAX;
+        ml[1] = 0.f;
+      }
+      break;  // the range ends here
+    }
+    load_tile<D, T>(a, seq, u.g * G, u.r, G, q_vec, tid, sm.q, sm.q_sum, sm.q_back, sm.q_seen);
+    __syncthreads();
+    {
       uint32_t qf[LW][4];
-      float f1[2], qs[2][NG];
+      float f1[2];
       int seen[2];
-      {
-        const int row = u.r * kRowsPerTile + gr, token = row / G;
-        const bool real = token < seq.count;
-        const T* src = static_cast<const T*>(a.q.data) + (seq.first + token) * a.q.token_stride +
-                       (u.g * G + row % G) * a.q.head_stride;
-        float x[LW][8], most = 0.f, sum[NG];
-        bool fine = true;
+      const uint32_t qs0 = sm.q_sum[0][gr][tq], qs1 = sm.q_sum[1][gr][tq], qs2 = sm.q_sum[2][gr][tq];
 #pragma unroll
-        for (int g = 0; g < NG; ++g) sum[g] = 0.f;
+      for (int i = 0; i < LW; ++i) *reinterpret_cast<uint4*>(qf[i]) = *reinterpret_cast<const uint4*>(sm.q[i][lane]);
 #pragma unroll
-        for (int i = 0; i < LW; ++i) {
-          const int dim = 64 * (i / 2) + 32 * (i % 2) + 8 * tq;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[i][e] = real ? kv4_to_float(src[dim + e]) : 0.f;
-            fine = fine && isfinite(x[i][e]);
-            most = fmaxf(most, fabsf(x[i][e]));
-            sum[i / 2] += x[i][e];
-          }
-        }
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        fine = __shfl_xor_sync(0xffffffffu, int(fine), 1) && fine;
-        fine = __shfl_xor_sync(0xffffffffu, int(fine), 2) && fine;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
-          sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
-          if (!fine) sum[g] = NAN;  // the row's logits are then all NaN
-        }
-        // |row| < 2^e: the row times 2^(14 - e) stays below 2^14
-        const int e = most > 0.f && fine ? int(__float_as_uint(most) >> 23) - 126 : 0;
-        const float up = pow2i((14 - e) / 2), up2 = pow2i(14 - e - (14 - e) / 2);
-#pragma unroll
-        for (int i = 0; i < LW; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float lift = j & 1 ? 0.0625f : 1.f;  // against the nibbles that carry 2^4
-            qf[i][j] = fine ? pack_f16(x[i][2 * j] * up * up2 * lift, x[i][2 * j + 1] * up * up2 * lift) : 0u;
-          }
-        const float factor = a.scale * 1.4426950408889634f;
-        // (q . n) 2^-24 2^(14 - e) -> logit in base 2
-        const float back = factor * pow2i((e + 10) / 2) * pow2i(e + 10 - (e + 10) / 2);
-        const int lim = real ? seq.len - seq.count + token + 1 : INT_MAX;  // rows past the last are not written
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int from = (2 * tq + c) * 4;
-          f1[c] = __shfl_sync(0xffffffffu, back, from);
-          seen[c] = __shfl_sync(0xffffffffu, lim, from);
-#pragma unroll
-          for (int g = 0; g < NG; ++g) qs[c][g] = __shfl_sync(0xffffffffu, sum[g], from) * factor;
-        }
+      for (int c = 0; c < 2; ++c) {
+        f1[c] = sm.q_back[2 * tq + c];
+        seen[c] = sm.q_seen[2 * tq + c];
       }
       const int least = __reduce_min_sync(0xffffffffu, min(seen[0], seen[1]));
 
@@ -427,24 +520,30 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
         for (int i = 0; i < 4; ++i) o[g][i][0] = o[g][i][1] = o[g][i][2] = o[g][i][3] = 0.f;
       }
 
-      for (; begin + warp + int64_t(done) * kWarps < u_end; ++done) {
-        const int stage = done % kStages;
-        if (!alive) continue;
+      const int first = int(u.at - begin) + kUnitPairs, rel_end = int(u_end - begin);
+      for (; place < rel_end; place += kWarps) {
+        const int done = place / kWarps, stage = done % kStages;
+        if (done % 32 == 0) {
+          look_up(done + 32 + lane);
+          __syncwarp();
+        }
+        const ulonglong2 from = *reinterpret_cast<const ulonglong2*>(sm.blocks[warp][done & 63]);
         if (!mbar_wait(&sm.full[warp][stage], done / kStages & 1, a.cache.status)) {
           alive = false;
-          continue;
+          place = INT_MAX / 2;  // leaves every loop
+          break;
         }
-        if (sm.absent[warp][stage]) {
+        if (!(from.x | from.y)) {
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.empty[warp][stage]);
+          if (lane == 0) issue(done + kStages, stage);
           continue;
         }
-        const uint8_t* blk = sm.ring[warp][stage];
-        // S^T: keys gr and gr + 8, rows 2 tq and 2 tq + 1
-        float acc[NG][4];
+        float s[4][2];  // [key][row]: keys gr and gr + 8 of each page, rows 2 tq and 2 tq + 1
+        alignas(16) uint32_t vm[4][NG];
 #pragma unroll
-        for (int g = 0; g < NG; ++g) acc[g][0] = acc[g][1] = acc[g][2] = acc[g][3] = 0.f;
-        {
+        for (int h = 0; h < 2; ++h) {
+          const uint8_t* blk = sm.ring[warp][stage][h];
+          float acc[NG][4], part[4];
           alignas(16) uint32_t w0[LW], w1[LW];
 #pragma unroll
           for (int i = 0; i < LW; i += L::kChunk) {
@@ -458,57 +557,52 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
               *reinterpret_cast<uint2*>(&w1[i]) = *reinterpret_cast<const uint2*>(p1);
             }
           }
+          const uint32_t m0 = *reinterpret_cast<const uint32_t*>(blk + L::k_meta(gr, tq % NG));
+          const uint32_t m1 = *reinterpret_cast<const uint32_t*>(blk + L::k_meta(gr + 8, tq % NG));
 #pragma unroll
-          for (int i = 0; i < LW; ++i) {
-            mma_f16(acc[i / 2], w0[i] & 0x000F000Fu, w1[i] & 0x000F000Fu, w0[i] & 0x00F000F0u, w1[i] & 0x00F000F0u, qf[i][0], qf[i][1]);
-            const uint32_t h0 = w0[i] >> 8, h1 = w1[i] >> 8;
-            mma_f16(acc[i / 2], h0 & 0x000F000Fu, h1 & 0x000F000Fu, h0 & 0x00F000F0u, h1 & 0x00F000F0u, qf[i][2], qf[i][3]);
-          }
-        }
-        alignas(16) uint32_t vm[2][NG];
-        float s[2][2];  // [key][row]
+          for (int j = 0; j < 4; ++j)  // word j / 2 of every group, its low or high bytes
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t* kp = reinterpret_cast<const uint32_t*>(blk + L::k_meta(gr + 8 * k, 0));
-          const uint32_t* vp = reinterpret_cast<const uint32_t*>(blk + L::v_meta(gr + 8 * k, 0));
-          alignas(16) uint32_t km[NG];
-          if constexpr (NG == 4) {
-            *reinterpret_cast<uint4*>(km) = *reinterpret_cast<const uint4*>(kp);
-            *reinterpret_cast<uint4*>(vm[k]) = *reinterpret_cast<const uint4*>(vp);
-          } else if constexpr (NG == 2) {
-            *reinterpret_cast<uint2*>(km) = *reinterpret_cast<const uint2*>(kp);
-            *reinterpret_cast<uint2*>(vm[k]) = *reinterpret_cast<const uint2*>(vp);
-          } else {
-            km[0] = kp[0];
-            vm[k][0] = vp[0];
-          }
-          float x0 = 0.f, x1 = 0.f, b0 = 0.f, b1 = 0.f;
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            x0 = fmaf(kv4_scale(km[g]), acc[g][2 * k], x0);
-            x1 = fmaf(kv4_scale(km[g]), acc[g][2 * k + 1], x1);
-            b0 = fmaf(kv4_bias(km[g]), qs[0][g], b0);
-            b1 = fmaf(kv4_bias(km[g]), qs[1][g], b1);
-          }
-          s[k][0] = fmaf(x0, f1[0], b0);
-          s[k][1] = fmaf(x1, f1[1], b1);
-        }
-        // keys behind a row's limit: no weight, and no step or bias that could be NaN
-        const int key0 = int(begin + warp + int64_t(done) * kWarps - u.at) * kPageTokens;
-        const bool edge = key0 + kPageTokens > least;
-        if (edge) {
+            for (int g = 0; g < NG; ++g) {
+              const int i = 2 * g + j / 2;
+              const uint32_t x = j & 1 ? w0[i] >> 8 : w0[i], y = j & 1 ? w1[i] >> 8 : w1[i];
+              if (j == 0) mma_f16_first(acc[g], x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, qf[i][0], qf[i][1]);
+              else mma_f16(acc[g], x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, qf[i][2 * (j & 1)], qf[i][2 * (j & 1) + 1]);
+            }
+          mma_bf16_first(part, m0, m1, m0, m1, qs0, qs1);
+          mma_bf16(part, m0, m1, m0, m1, qs2, 0u);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
+            alignas(16) uint32_t km[NG];
+            load_words<NG>(km, blk + L::k_meta(gr + 8 * k, 0));
+            load_words<NG>(vm[2 * h + k], blk + L::v_meta(gr + 8 * k, 0));
+            float x0 = kv4_scale(km[0]) * acc[0][2 * k], x1 = kv4_scale(km[0]) * acc[0][2 * k + 1];
+#pragma unroll
+            for (int g = 1; g < NG; ++g) {
+              x0 = fmaf(kv4_scale(km[g]), acc[g][2 * k], x0);
+              x1 = fmaf(kv4_scale(km[g]), acc[g][2 * k + 1], x1);
+            }
+            s[2 * h + k][0] = fmaf(x0, f1[0], part[2 * k]);
+            s[2 * h + k][1] = fmaf(x1, f1[1], part[2 * k + 1]);
+          }
+        }
+        // keys behind a row's limit and pages that are not there: no weight, and no step or bias that could be NaN
+        const int key0 = (place - first) * 2 * kPageTokens;
+        const bool edge = key0 + 2 * kPageTokens > least || !from.x || !from.y;
+        if (edge) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
             const int key = key0 + gr + 8 * k;
-            if (key >= seen[0]) s[k][0] = -INFINITY;
-            if (key >= seen[1]) s[k][1] = -INFINITY;
-            if (key >= seq.len) {
+            const bool there = k < 2 ? from.x != 0 : from.y != 0;
+            if (!there || key >= seen[0]) s[k][0] = -INFINITY;
+            if (!there || key >= seen[1]) s[k][1] = -INFINITY;
+            if (!there || key >= seq.len) {
 #pragma unroll
               for (int g = 0; g < NG; ++g) vm[k][g] = 0u;
             }
           }
         }
-        const float h0 = fmaxf(s[0][0], s[1][0]), h1 = fmaxf(s[0][1], s[1][1]);
+        const float h0 = fmaxf(fmaxf(s[0][0], s[1][0]), fmaxf(s[2][0], s[3][0]));
+        const float h1 = fmaxf(fmaxf(s[0][1], s[1][1]), fmaxf(s[2][1], s[3][1]));
         if (__any_sync(0xffffffffu, h0 > m[0] + kLazy || h1 > m[1] + kLazy)) {
           float top[2] = {h0, h1};
 #pragma unroll
@@ -531,24 +625,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
             }
           }
         }
-        float p[2][2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            p[k][c] = exp2_fast(s[k][c] - m[c]);
-            l[c] += p[k][c];
-          }
         // V's steps to at most 2^6
         float big = 0.f;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) big = fmaxf(big, fmaxf(kv4_scale(vm[0][g]), kv4_scale(vm[1][g])) * vinv[g]);
+        for (int g = 0; g < NG; ++g)
+          big = fmaxf(big, vinv[g] * fmaxf(fmaxf(kv4_scale(vm[0][g]), kv4_scale(vm[1][g])), fmaxf(kv4_scale(vm[2][g]), kv4_scale(vm[3][g]))));
         if (__any_sync(0xffffffffu, big > 64.f)) {
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
-            const float top = warp_max(fmaxf(kv4_scale(vm[0][g]), kv4_scale(vm[1][g])));
+            const float top = warp_max(fmaxf(fmaxf(kv4_scale(vm[0][g]), kv4_scale(vm[1][g])), fmaxf(kv4_scale(vm[2][g]), kv4_scale(vm[3][g]))));
             const float fresh = fminf(vinv[g], pow2i(min(126, 132 - int(__float_as_uint(top) >> 23))));
-            const float f = fresh / vinv[g];
+            const float f = pow2i(int(__float_as_uint(fresh) >> 23) - int(__float_as_uint(vinv[g]) >> 23));
             vinv[g] = fresh;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -559,46 +646,61 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
             }
           }
         }
-        uint32_t pb[NG][2];
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float step = kv4_scale(vm[k][g]) * vinv[g], bias = kv4_bias(vm[k][g]);
-            pb[g][k] = transpose8x8(pack_f16(p[k][0] * step, p[k][1] * step));
-            if (edge) {  // a bias that is NaN counts only for the rows that see its key
-              if (key0 + gr + 8 * k < seen[0]) extra[0][g] = fmaf(p[k][0], bias, extra[0][g]);
-              if (key0 + gr + 8 * k < seen[1]) extra[1][g] = fmaf(p[k][1], bias, extra[1][g]);
-            } else {
-              extra[0][g] = fmaf(p[k][0], bias, extra[0][g]);
-              extra[1][g] = fmaf(p[k][1], bias, extra[1][g]);
+          for (int c = 0; c < 2; ++c) {
+            s[k][c] = exp2_fast(s[k][c] - m[c]);
+            l[c] += s[k][c];
+          }
+        if (edge) {  // a bias that is NaN counts only for the rows that see its key
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              const float bias = kv4_bias(vm[k][g]);
+              extra[0][g] = fmaf(s[k][0], key0 + gr + 8 * k < seen[0] ? bias : 0.f, extra[0][g]);
+              extra[1][g] = fmaf(s[k][1], key0 + gr + 8 * k < seen[1] ? bias : 0.f, extra[1][g]);
             }
-          }
-        {
-          // nibbles of keys 2 tq, 2 tq + 1 (even places first) and 2 tq + 8, 2 tq + 9
-          alignas(16) uint32_t w[4][NG];
-          const uint8_t* pv = blk + L::kV + (gr / L::kRows * kPageTokens + tq) * 32 + gr % L::kRows * (D / 16);
+        } else {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint8_t* q = pv + ((k & 1) * 8 + (k >> 1) * 4) * 32;
-            if constexpr (NG == 4) *reinterpret_cast<uint4*>(w[k]) = *reinterpret_cast<const uint4*>(q);
-            else if constexpr (NG == 2) *reinterpret_cast<uint2*>(w[k]) = *reinterpret_cast<const uint2*>(q);
-            else w[k][0] = *reinterpret_cast<const uint32_t*>(q);
-          }
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              const float bias = kv4_bias(vm[k][g]);
+              extra[0][g] = fmaf(s[k][0], bias, extra[0][g]);
+              extra[1][g] = fmaf(s[k][1], bias, extra[1][g]);
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t pb[NG][2];
 #pragma unroll
           for (int g = 0; g < NG; ++g)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t x = __byte_perm(w[0][g], w[1][g], h ? 0x7632 : 0x5410);
-              uint32_t y = __byte_perm(w[2][g], w[3][g], h ? 0x7632 : 0x5410);
-              mma_f16(o[g][2 * h], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, pb[g][0], pb[g][1]);
+            for (int k = 0; k < 2; ++k) {
+              const float step = kv4_scale(vm[2 * h + k][g]) * vinv[g];
+              pb[g][k] = transpose8x8(pack_f16(s[2 * h + k][0] * step, s[2 * h + k][1] * step));
+            }
+          // nibbles of keys 2 tq, 2 tq + 1 (even places first) and 2 tq + 8, 2 tq + 9
+          alignas(16) uint32_t w[4][NG];
+          const uint8_t* pv = sm.ring[warp][stage][h] + L::kV + (gr / L::kRows * kPageTokens + tq) * 32 + gr % L::kRows * (D / 16);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) load_words<NG>(w[k], pv + ((k & 1) * 8 + (k >> 1) * 4) * 32);
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              uint32_t x = __byte_perm(w[0][g], w[1][g], b ? 0x7632 : 0x5410);
+              uint32_t y = __byte_perm(w[2][g], w[3][g], b ? 0x7632 : 0x5410);
+              mma_f16(o[g][2 * b], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, pb[g][0], pb[g][1]);
               x >>= 8;
               y >>= 8;
-              mma_f16(o[g][2 * h + 1], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, pb[g][0], pb[g][1]);
+              mma_f16(o[g][2 * b + 1], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, pb[g][0], pb[g][1]);
             }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.empty[warp][stage]);
+        if (lane == 0) issue(done + kStages, stage);
       }
 
       // join the warps: row maxima and sums, then the rows one warp at a time
@@ -615,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
           sm.ml[warp][2 * tq + c][1] = l[c];
         }
       }
-      consumers_sync();
+      __syncthreads();
       float f[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -624,33 +726,51 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
         for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm.ml[w][2 * tq + c][0]);
         f[c] = exp2_fast(m[c] - M);
       }
-      for (int w = 0; w < kWarps; ++w) {
-        if (w == warp) {
+      // gates of the rows this thread will write
+      constexpr int kItems = kRowsPerTile * (D / 8) / kThreads > 0 ? kRowsPerTile * (D / 8) / kThreads : 1;
+      float gate[kItems][8];
+      if (whole && a.gate.data) {
 #pragma unroll
-          for (int g = 0; g < NG; ++g)
+        for (int k = 0; k < kItems; ++k) {
+          const int e = tid + k * kThreads, row = u.r * kRowsPerTile + e / (D / 8), token = row / G;
+          if (e < kRowsPerTile * (D / 8) && token < seq.count)
+            load_gate(a, seq.first + token, u.g * G + row % G, e % (D / 8) * 8, gate[k]);
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {  // warps 0, 1 store, then 2, 3 add
+        if (warp / 2 == half) {
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            const float back = pow2i(24 + 127 - int(__float_as_uint(vinv[g]) >> 23));  // 2^24 over the power on V's steps
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              float* row = &sm.o[2 * tq + c][64 * g + 8 * gr];
-              const float back = 16777216.f / vinv[g];  // 2^24 over the power on V's steps
+              float* row = &sm.o[warp % 2][2 * tq + c][64 * g + 8 * gr];
               float y[8];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 y[2 * i] = fmaf(o[g][i][c], back, extra[c][g]) * f[c];
                 y[2 * i + 1] = fmaf(o[g][i][2 + c], back * 0.0625f, extra[c][g]) * f[c];
               }
-              if (w > 0) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] += row[i];
+              for (int i = 0; i < 2; ++i) {
+                float4 v = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+                float4* at = reinterpret_cast<float4*>(row) + i;
+                if (half) {
+                  const float4 old = *at;
+                  v = make_float4(old.x + v.x, old.y + v.y, old.z + v.z, old.w + v.w);
+                }
+                *at = v;
               }
-#pragma unroll
-              for (int i = 0; i < 2; ++i) reinterpret_cast<float4*>(row)[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
             }
+          }
         }
-        consumers_sync();
+        __syncthreads();
       }
-      const bool whole = u.at >= begin && u.at + pages <= end;
-      const int slot = u_begin == begin ? 0 : 1;
-      for (int e = tid; e < kRowsPerTile * (D / 8); e += kWarps * 32) {
+#pragma unroll
+      for (int k = 0; k < kItems; ++k) {
+        const int e = tid + k * kThreads;
+        if (e >= kRowsPerTile * (D / 8)) break;
         const int rr = e / (D / 8), dim = e % (D / 8) * 8;
         float M = -FLT_MAX, sum = 0.f, y[8];
 #pragma unroll
@@ -658,14 +778,21 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) sum += sm.ml[w][rr][1] * exp2_fast(sm.ml[w][rr][0] - M);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = sm.o[rr][dim + i];
+        for (int i = 0; i < 8; i += 4) {
+          const float4 p = *reinterpret_cast<const float4*>(&sm.o[0][rr][dim + i]);
+          const float4 q = *reinterpret_cast<const float4*>(&sm.o[1][rr][dim + i]);
+          y[i] = p.x + q.x;
+          y[i + 1] = p.y + q.y;
+          y[i + 2] = p.z + q.z;
+          y[i + 3] = p.w + q.w;
+        }
         if (whole) {
           const int row = u.r * kRowsPerTile + rr, token = row / G;
           if (token >= seq.count) continue;
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
           for (int i = 0; i < 8; ++i) y[i] *= inv;
-          write_dims<T>(a, seq.first + token, u.g * G + row % G, dim, y, out_vec);
+          write_dims<T>(a, seq.first + token, u.g * G + row % G, dim, y, gate[k], out_vec);
           if (dim == 0 && a.lse)
             a.lse[size_t(seq.first + token) * a.cache.Hq + u.g * G + row % G] =
                 sum == 0.f ? -INFINITY : (M + log2f(sum)) * 0.6931471805599453f;
@@ -680,61 +807,113 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
           }
         }
       }
-      consumers_sync();
-      if (u_end == end) break;
-      advance(u, seq, pages);
     }
+    if (u_end == end) break;
+    __syncthreads();
+    advance(u, seq, length);
+  }
+  if (!alive && lane == 0) {
+    // a wait ran out: let copies in flight land before the CTA leaves
+    for (int i = 0; i < 2 * kStages; ++i) mbar_wait(&sm.full[warp][i % kStages], i / kStages, a.cache.status);
   }
 }
 
 // Joins the partial results of a unit whose pages span several CTAs, and
-// writes the rows of a unit that has no page. One CTA per unit.
+// writes the rows of a unit that has no page. One CTA per unit; a warp per row
+// weighs the parts, then the threads sum them.
+constexpr int kMergeParts = 64;  // weighed at a time
 template <int D, class T>
 __global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4AttentionArgs a, int ctas, int tiles, bool out_vec) {
   pdl_trigger();
   pdl_wait();
-  const int Hkv = a.cache.Hkv, G = a.cache.Hq / Hkv;
+  __shared__ float weight[kRowsPerTile][kMergeParts], row_m[kRowsPerTile], row_l[kRowsPerTile];
+  const int Hkv = a.cache.Hkv, G = a.cache.Hq / Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = blockIdx.x % tiles, g = blockIdx.x / tiles % Hkv, s = blockIdx.x / tiles / Hkv;
+  const Workspace ws = carve(a.workspace, a.n_seq, ctas);
+  const int64_t first = ws.offsets[s], next = ws.offsets[s + 1], range = *ws.range;
   const Seq seq = load_seq(a, s, G, false);
   if (r >= seq.tiles) return;
-  const Workspace ws = carve(a.workspace, a.n_seq, ctas);
-  int64_t at = ws.offsets[s] + g * ((ws.offsets[s + 1] - ws.offsets[s]) / Hkv);
-  for (int i = 0; i < r; ++i) at += tile_pages(seq, i, G);
-  const int pages = tile_pages(seq, r, G);
-  const int64_t range = *ws.range;
-  const int64_t c0 = at / range, c1 = pages ? (at + pages - 1) / range : c0;
-  if (pages && c0 == c1) return;  // whole in one CTA
-  for (int e = threadIdx.x; e < kRowsPerTile * (D / 8); e += blockDim.x) {
-    const int rr = e / (D / 8), dim = e % (D / 8) * 8, row = r * kRowsPerTile + rr, token = row / G;
-    if (token >= seq.count) continue;
-    float M = -FLT_MAX, sum = 0.f, y[8] = {};
-    if (pages) {
-      for (int64_t c = c0; c <= c1; ++c) {
-        const size_t slot = (size_t(c) * 2 + (max(at, c * range) == c * range ? 0 : 1)) * kRowsPerTile + rr;
-        const float2 ml = *reinterpret_cast<const float2*>(ws.ml + slot * 2);
-        const float4 lo = *reinterpret_cast<const float4*>(ws.o + slot * D + dim);
-        const float4 hi = *reinterpret_cast<const float4*>(ws.o + slot * D + dim + 4);
-        const float top = fmaxf(M, ml.x), f0 = exp2_fast(M - top), f1 = exp2_fast(ml.x - top);
-        M = top;
-        sum = sum * f0 + ml.y * f1;
-        y[0] = y[0] * f0 + lo.x * f1;
-        y[1] = y[1] * f0 + lo.y * f1;
-        y[2] = y[2] * f0 + lo.z * f1;
-        y[3] = y[3] * f0 + lo.w * f1;
-        y[4] = y[4] * f0 + hi.x * f1;
-        y[5] = y[5] * f0 + hi.y * f1;
-        y[6] = y[6] * f0 + hi.z * f1;
-        y[7] = y[7] * f0 + hi.w * f1;
+  int64_t at = first + g * ((next - first) / Hkv);
+  for (int i = 0; i < r; ++i) at += unit_length(seq, i, G);
+  const int length = unit_length(seq, r, G);
+  const int64_t c0 = at / range, c1 = length ? (at + length - 1) / range : c0 - 1;
+  if (length && c0 == c1) return;  // whole in one CTA
+  // a CTA's first unit is in its slot 0, another that ends behind it in slot 1
+  const auto part = [&](int64_t c) { return size_t(c * 2 + (at > c * range ? 1 : 0)) * kRowsPerTile; };
+  constexpr int kItems = kRowsPerTile * (D / 8) / 256 > 0 ? kRowsPerTile * (D / 8) / 256 : 1;
+  const int rr = threadIdx.x / (D / 8), dim = threadIdx.x % (D / 8) * 8;
+  static_assert(kItems == 1 && kRowsPerTile == 8, "a thread writes 8 dims of one row");
+  const int row = r * kRowsPerTile + rr, token = row / G;
+  const bool mine = rr < kRowsPerTile && token < seq.count;
+  float gate[8], y[8] = {};
+  if (mine && a.gate.data) load_gate(a, seq.first + token, g * G + row % G, dim, gate);
+  float M = -FLT_MAX, sum = 0.f;
+  for (int64_t c = c0; c <= c1; c += kMergeParts) {
+    const int n = int(min(c1 - c + 1, int64_t(kMergeParts)));
+    float m[kMergeParts / 32], l[kMergeParts / 32], top = M;
+#pragma unroll
+    for (int k = 0; k < kMergeParts / 32; ++k) {
+      const int i = lane + 32 * k;
+      m[k] = -FLT_MAX;
+      l[k] = 0.f;
+      if (i < n) {
+        const float2 ml = *reinterpret_cast<const float2*>(ws.ml + (part(c + i) + warp) * 2);
+        m[k] = ml.x;
+        l[k] = ml.y;
+      }
+      top = fmaxf(top, m[k]);
+    }
+    top = warp_max(top);
+    const float old = exp2_fast(M - top);
+    float add = 0.f;
+#pragma unroll
+    for (int k = 0; k < kMergeParts / 32; ++k) {
+      const float w = exp2_fast(m[k] - top);
+      add += l[k] * w;
+      weight[warp][lane + 32 * k] = l[k] == 0.f ? 0.f : w;  // a part that saw no key may hold anything
+    }
+    sum = sum * old + warp_sum(add);
+    M = top;
+    if (lane == 0) row_m[warp] = old;
+    __syncthreads();
+    if (mine) {
+      const float f = row_m[rr];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] *= f;
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float w = weight[rr][i];
+        const float* p = ws.o + (part(c + i) + rr) * D + dim;
+        const float4 lo = *reinterpret_cast<const float4*>(p), hi = *reinterpret_cast<const float4*>(p + 4);
+        if (w != 0.f) {
+          y[0] = fmaf(lo.x, w, y[0]);
+          y[1] = fmaf(lo.y, w, y[1]);
+          y[2] = fmaf(lo.z, w, y[2]);
+          y[3] = fmaf(lo.w, w, y[3]);
+          y[4] = fmaf(hi.x, w, y[4]);
+          y[5] = fmaf(hi.y, w, y[5]);
+          y[6] = fmaf(hi.z, w, y[6]);
+          y[7] = fmaf(hi.w, w, y[7]);
+        }
       }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] *= inv;
-    write_dims<T>(a, seq.first + token, g * G + row % G, dim, y, out_vec);
-    if (dim == 0 && a.lse)
-      a.lse[size_t(seq.first + token) * a.cache.Hq + g * G + row % G] =
-          sum == 0.f ? -INFINITY : (M + log2f(sum)) * 0.6931471805599453f;
+    __syncthreads();
   }
+  if (lane == 0) {
+    row_m[warp] = M;
+    row_l[warp] = sum;
+  }
+  __syncthreads();
+  if (!mine) return;
+  M = row_m[rr];
+  sum = row_l[rr];
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] *= inv;
+  write_dims<T>(a, seq.first + token, g * G + row % G, dim, y, gate, out_vec);
+  if (dim == 0 && a.lse)
+    a.lse[size_t(seq.first + token) * a.cache.Hq + g * G + row % G] =
+        sum == 0.f ? -INFINITY : (M + log2f(sum)) * 0.6931471805599453f;
 }
 
 // Lane's dims lane E .. lane E + E - 1 of K of one cached token.
@@ -791,11 +970,12 @@ void attend(const Kv4AttentionArgs& a, cudaStream_t s) {
   Kv4AttentionArgs b = a;
   const int G = a.cache.Hq / a.cache.Hkv, ctas = a.sm_count * kCtasPerSm;
   const int tiles = (a.max_count * G + kRowsPerTile - 1) / kRowsPerTile;
+  const bool q_vec = reinterpret_cast<uintptr_t>(a.q.data) % 16 == 0 && a.q.token_stride % 8 == 0 && a.q.head_stride % 8 == 0;
   const bool vec = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_token_stride % 8 == 0 && a.out_head_stride % 8 == 0;
   if (a.weights_out && !a.lse)
     b.lse = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) +
                                      kv4_workspace_bytes(a.cache.Hq, a.cache.Hkv, D, a.n_seq, 0, a.sm_count));
-  launch_pdl(kv4_decode_kernel<D, T>, ctas, kThreads, sizeof(Smem<D>), s, b, vec);
+  launch_pdl(kv4_decode_kernel<D, T>, ctas, kThreads, sizeof(Smem<D>), s, b, q_vec, vec);
   count_launch();
   launch_pdl(kv4_merge_kernel<D, T>, dim3(unsigned(a.n_seq * a.cache.Hkv * tiles)), 256, 0, s, b, ctas, tiles, vec);
   count_launch();

@@ -1,0 +1,174 @@
+// Device helpers shared by the kernels that read the 4-bit KV cache.
+#pragma once
+#include <cfloat>
+#include <climits>
+
+#include "kernels.h"
+#include "kv4.h"
+
+namespace qwen {
+namespace {
+
+constexpr int kRowsPerTile = 8;  // query rows of an MMA tile
+constexpr long long kWaitCycles = 2000000000ll;
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32_t* status) {
+  if (mbar_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (;;) {
+    if (mbar_try(bar, parity)) return true;
+    if (clock64() - t0 > kWaitCycles) {
+      kv4_flag(status, kErrTimeout);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// d = a b from zero accumulators (no registers to clear)
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
+  if constexpr (N == 4) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
+  else if constexpr (N == 2) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+  else w[0] = *reinterpret_cast<const uint32_t*>(p);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float(uint32_t(min(max(e, -126), 127) + 127) << 23); }
+
+// Length of sequence s, kept within the table and, when weights are written, their rows.
+__device__ __forceinline__ int kv4_length(const Kv4AttentionArgs& a, int s, bool report) {
+  int64_t most = a.table_stride * kPageTokens;
+  if (a.weights_out) most = min(most, a.weights_stride);
+  const int len = a.kv_lens[s];
+  if (len < 0 || len > most) {
+    if (report) kv4_flag(a.cache.status, kErrBounds);
+    return int(min(max(int64_t(len), int64_t(0)), most));
+  }
+  return len;
+}
+
+// A sequence's query rows (token-major: row = token * G + head of the group)
+// and keys; the row range is kept inside the call's tokens.
+struct Seq {
+  int first, count, len, tiles;
+};
+__device__ __forceinline__ Seq load_seq(const Kv4AttentionArgs& a, int s, int G, bool report) {
+  Seq q;
+  q.first = min(max(a.cu_seqlens[s], 0), a.tokens);
+  q.count = min(max(a.cu_seqlens[s + 1], 0), a.tokens) - q.first;
+  q.len = kv4_length(a, s, report);
+  if (q.count < 0 || q.count > a.max_count) {
+    if (report) kv4_flag(a.cache.status, kErrBounds);
+    q.count = 0;
+  }
+  q.tiles = (q.count * G + kRowsPerTile - 1) / kRowsPerTile;
+  return q;
+}
+// Keys that the last row of tile r sees, and the pages that hold them.
+__device__ __forceinline__ int tile_pages(const Seq& q, int r, int G) {
+  const int token = min(q.count - 1, ((r + 1) * kRowsPerTile - 1) / G);
+  return max(0, q.len - q.count + token + 1 + kPageTokens - 1) / kPageTokens;
+}
+
+// Sigmoid by the approximate reciprocal: a relative error of a few 2^-23, far below a 16-bit result's rounding.
+__device__ __forceinline__ float sigmoid_fast(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+
+// Eight dims of one output row and its gate.
+__device__ __forceinline__ void load_gate(const Kv4AttentionArgs& a, int token, int head, int dim, bool vec, float (&g)[8]) {
+  const float* p = static_cast<const float*>(a.gate.data) + token * a.gate.token_stride + head * a.gate.head_stride + dim;
+  if (vec) {
+    const float4 lo = *reinterpret_cast<const float4*>(p), hi = *reinterpret_cast<const float4*>(p + 4);
+    g[0] = lo.x, g[1] = lo.y, g[2] = lo.z, g[3] = lo.w, g[4] = hi.x, g[5] = hi.y, g[6] = hi.z, g[7] = hi.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] = p[i];
+  }
+}
+template <class T>
+__device__ __forceinline__ void write_dims(const Kv4AttentionArgs& a, int token, int head, int dim, float (&y)[8],
+                                           const float (&gate)[8], bool vec) {
+  if (a.gate.data) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] *= sigmoid_fast(gate[i]);
+  }
+  T* out = static_cast<T*>(a.out) + token * a.out_token_stride + head * a.out_head_stride + dim;
+  alignas(16) T v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = kv4_from_float<T>(y[i]);
+  if (vec) {
+    *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = v[i];
+  }
+}
+
+}  // namespace
+}  // namespace qwen

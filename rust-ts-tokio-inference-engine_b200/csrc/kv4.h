@@ -2,6 +2,8 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <climits>
+
 #include "common.cuh"
 
 namespace qwen {
@@ -109,7 +111,11 @@ struct Kv4AttentionArgs {
   void* workspace = nullptr;
   size_t workspace_bytes = 0;
   int sm_count = 0;
+  int row_limit = INT_MAX;  // sequences with more query rows per KV head run in kv4_chunk.cu
 };
+// Sequences above row_limit, tcgen05 tiles of 128 rows (no lse, no weights).
+size_t kv4_chunk_workspace_bytes(int Hq, int Hkv, int D, size_t n_seq, size_t tokens, int sm_count);
+void launch_kv4_chunk(const Kv4AttentionArgs& a, void* workspace, cudaStream_t s);
 size_t kv4_workspace_bytes(int Hq, int Hkv, int D, size_t n_seq, size_t tokens, int sm_count);
 void launch_kv4_attention(const Kv4AttentionArgs& a, cudaStream_t s);
 

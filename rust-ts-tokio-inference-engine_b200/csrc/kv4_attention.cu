@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
   auto seq_at = [&](int s) {
     if (per > 1) return load_seq(a, s, G, false);
     Seq q{sm.first[s], sm.count[s], sm.len[s], 0};
-    q.tiles = (q.count * G + kRowsPerTile - 1) / kRowsPerTile;
+    q.tiles = q.count * G > a.row_limit ? 0 : (q.count * G + kRowsPerTile - 1) / kRowsPerTile;
     return q;
   };
   if (blockIdx.x == gridDim.x - 1) {  // for the merge
@@ -354,10 +354,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
         __syncwarp();
       }
       const ulonglong2 from = *reinterpret_cast<const ulonglong2*>(sm.blocks[warp][done & 63]);
-      if (!mbar_wait(&sm.full[warp][stage], done / kStages & 1, a.cache.status)) {
+      if (!kv4_wait(&sm.full[warp][stage], done / kStages & 1, a.cache.status)) {
         // a wait ran out: let the copies in flight land before leaving
         if (lane == 0)
-          for (int i = 0; i < 2 * kStages; ++i) mbar_wait(&sm.full[warp][i % kStages], i / kStages, a.cache.status);
+          for (int i = 0; i < 2 * kStages; ++i) kv4_wait(&sm.full[warp][i % kStages], i / kStages, a.cache.status);
         return;
       }
       if (!(from.x | from.y)) {
@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(Kv4AttentionAr
   const Workspace ws = carve(a.workspace, unit_entries(a.tokens, a.n_seq, G, Hkv), workers);
   const Seq seq = load_seq(a, s, G, false);
   const int row = r * kRowsPerTile + rr, token = row / G, head = g * G + row % G;
-  if (token >= seq.count) return;  // a tile without rows has no entry either
+  if (r >= seq.tiles || token >= seq.count) return;  // a tile without rows has no entry either
   const int2 unit = ws.units[unit_index(seq, s, r, g, G, Hkv)];
   const int n = unit.y;
   if (n == 1) return;  // whole in one warp
@@ -728,7 +728,15 @@ __global__ void __launch_bounds__(128) kv4_weights_kernel(Kv4AttentionArgs a, co
   }
 }
 
-void count_launch() { g_kernel_launches.fetch_add(1, std::memory_order_relaxed); }
+size_t decode_workspace(int Hq, int Hkv, int D, size_t n_seq, size_t tokens, int sm_count) {
+  return align16(unit_entries(tokens, n_seq, Hq / Hkv, Hkv) * 8) +
+         size_t(sm_count) * kCtasPerSm * kWarps * 2 * kRowsPerTile * (D + 2) * 4;
+}
+
+// Rows of a sequence up to which it runs here when neither lse nor weights are
+// asked for: two tiles, which this kernel reads the pages for twice; from three
+// on the 128-row tiles of kv4_chunk_kernel are faster.
+constexpr int kChunkRows = 16;
 
 template <int D, class T>
 void attend(const Kv4AttentionArgs& a, cudaStream_t s) {
@@ -738,7 +746,9 @@ void attend(const Kv4AttentionArgs& a, cudaStream_t s) {
   });
   Kv4AttentionArgs b = a;
   const int G = a.cache.Hq / a.cache.Hkv, ctas = a.sm_count * kCtasPerSm;
-  const int tiles = (a.max_count * G + kRowsPerTile - 1) / kRowsPerTile;
+  const bool chunks = !a.lse && !a.weights_out && a.max_count * int64_t(G) > kChunkRows;
+  b.row_limit = chunks ? kChunkRows : INT_MAX;
+  const int tiles = (int(std::min(int64_t(a.max_count) * G, int64_t(b.row_limit))) + kRowsPerTile - 1) / kRowsPerTile;
   if (int64_t(a.n_seq) * a.cache.Hkv * tiles > (int64_t(1) << 30) / (a.table_stride / 2 + 1 + kUnitPairs))
     throw std::invalid_argument("kv4 attention: n_seq x kv_heads x query tiles x pages beyond 2^31; split the call");
   const bool q_vec = reinterpret_cast<uintptr_t>(a.q.data) % 16 == 0 && a.q.token_stride % 8 == 0 && a.q.head_stride % 8 == 0;
@@ -748,22 +758,22 @@ void attend(const Kv4AttentionArgs& a, cudaStream_t s) {
     b.lse = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + a.workspace_bytes / 16 * 16 -
                                      align16(size_t(a.tokens) * a.cache.Hq * 4));  // the workspace's end
   launch_pdl(kv4_decode_kernel<D, T>, ctas, kThreads, sizeof(Smem<D>), s, b, q_vec, gate_vec, vec);
-  count_launch();
-  launch_pdl(kv4_merge_kernel<D, T>, dim3(unsigned(a.n_seq * a.cache.Hkv * tiles), std::min(kRowsPerTile, a.max_count * G)), kMergeThreads, 0, s, b,
-             ctas * kWarps, tiles);
-  count_launch();
+  launch_pdl(kv4_merge_kernel<D, T>, dim3(unsigned(a.n_seq * a.cache.Hkv * tiles), std::min(int64_t(kRowsPerTile), int64_t(a.max_count) * G)),
+             kMergeThreads, 0, s, b, ctas * kWarps, tiles);
+  g_kernel_launches.fetch_add(2, std::memory_order_relaxed);
+  if (chunks) launch_kv4_chunk(b, static_cast<uint8_t*>(a.workspace) + decode_workspace(a.cache.Hq, a.cache.Hkv, D, a.n_seq, a.tokens, a.sm_count), s);
   if (a.weights_out) {
     launch_pdl(kv4_weights_kernel<D, T>, dim3(unsigned(a.table_stride), a.n_seq * a.cache.Hkv), 128, 0, s, b,
                static_cast<const float*>(b.lse));
-    count_launch();
+    g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
   }
 }
 
 }  // namespace
 
 size_t kv4_workspace_bytes(int Hq, int Hkv, int D, size_t n_seq, size_t tokens, int sm_count) {
-  return align16(unit_entries(tokens, n_seq, Hq / Hkv, Hkv) * 8) +
-         size_t(sm_count) * kCtasPerSm * kWarps * 2 * kRowsPerTile * (D + 2) * 4 + align16(tokens * size_t(Hq) * 4);
+  return decode_workspace(Hq, Hkv, D, n_seq, tokens, sm_count) + kv4_chunk_workspace_bytes(Hq, Hkv, D, n_seq, tokens, sm_count) +
+         align16(tokens * size_t(Hq) * 4);
 }
 
 void launch_kv4_attention(const Kv4AttentionArgs& a, cudaStream_t s) {

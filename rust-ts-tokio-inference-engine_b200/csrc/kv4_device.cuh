@@ -5,49 +5,38 @@
 
 #include "kernels.h"
 #include "kv4.h"
+#include "tcgen05.cuh"
 
 namespace qwen {
 namespace {
 
 constexpr int kRowsPerTile = 8;  // query rows of an MMA tile
-constexpr long long kWaitCycles = 2000000000ll;
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32_t* status) {
+// Bounded waits on a barrier; a wait that runs out (about a second) sets the
+// status bit and, where the CTA has roles that wait for one another, `abort`,
+// which ends the other roles' waits too.
+__device__ __forceinline__ bool kv4_wait(uint64_t* bar, uint32_t parity, uint32_t* status, volatile int* abort = nullptr) {
   if (mbar_try(bar, parity)) return true;
   const long long t0 = clock64();
   for (;;) {
-    if (mbar_try(bar, parity)) return true;
+    if (mbar_try_sleep(bar, parity, 2000)) return true;
+    if (abort && *abort) return false;
     if (clock64() - t0 > kWaitCycles) {
       kv4_flag(status, kErrTimeout);
+      if (abort) *abort = 1;
       return false;
     }
   }
 }
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* v) {
   asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]),
+        "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]),
+        "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -117,7 +106,7 @@ __device__ __forceinline__ int kv4_length(const Kv4AttentionArgs& a, int s, bool
 // A sequence's query rows (token-major: row = token * G + head of the group)
 // and keys; the row range is kept inside the call's tokens.
 struct Seq {
-  int first, count, len, tiles;
+  int first, count, len, tiles;  // tiles of 8 rows; none for a sequence with more rows than the call's row_limit
 };
 __device__ __forceinline__ Seq load_seq(const Kv4AttentionArgs& a, int s, int G, bool report) {
   Seq q;
@@ -128,7 +117,7 @@ __device__ __forceinline__ Seq load_seq(const Kv4AttentionArgs& a, int s, int G,
     if (report) kv4_flag(a.cache.status, kErrBounds);
     q.count = 0;
   }
-  q.tiles = (q.count * G + kRowsPerTile - 1) / kRowsPerTile;
+  q.tiles = q.count * G > a.row_limit ? 0 : (q.count * G + kRowsPerTile - 1) / kRowsPerTile;
   return q;
 }
 // Keys that the last row of tile r sees, and the pages that hold them.

@@ -209,6 +209,9 @@ def test_ragged_counts(pkg, heads, counts, lens):
     win = torch.rand(len(lens), seqs.Hkv, width, generator=seqs.gen, device="cuda")
     out, lse, weights = attend(pkg, seqs, q, cu, counts, stats=True, weights_in=win)
     check_attention(seqs, q, host, out, lse, weights, weights_in=win)
+    plain, _, _ = attend(pkg, seqs, q, cu, counts)
+    check_attention(seqs, q, host, plain)
+    assert (plain[host[-1]:] == 77).all()
     assert (out[host[-1]:] == 77).all() and (lse[host[-1]:] == 77).all()  # rows behind the last sequence
     for s, n in enumerate(lens):
         assert (weights[s, :, n:] == 55).all()
@@ -223,8 +226,10 @@ def test_rows_that_see_no_key(pkg, heads):
     q, cu, host = seqs.queries(counts, torch.float16)
     out, lse, weights = attend(pkg, seqs, q, cu, counts, stats=True)
     check_attention(seqs, q, host, out, lse, weights)
+    plain, _, _ = attend(pkg, seqs, q, cu, counts)
+    check_attention(seqs, q, host, plain)
     for row in (0, 1, 5, 6, 7, 8, 9, 10):
-        assert (out[row] == 0).all() and (lse[row] == -math.inf).all()
+        assert (out[row] == 0).all() and (lse[row] == -math.inf).all() and (plain[row] == 0).all()
 
 
 @pytest.mark.parametrize("spread,scale", [(30.0, 0.0), (1.0, 8.0), (1e-4, 0.25), (3e4, 1e-6)])
@@ -234,6 +239,9 @@ def test_large_and_small_logits(pkg, heads, spread, scale):
     q, cu, host = seqs.queries([1, 3], torch.bfloat16)
     out, lse, weights = attend(pkg, seqs, q, cu, [1, 3], stats=True, scale=scale)
     check_attention(seqs, q, host, out, lse, weights, scale=scale)
+    q, cu, host = seqs.queries([30, 70], torch.float16)
+    out, _, _ = attend(pkg, seqs, q, cu, [30, 70], scale=scale)
+    check_attention(seqs, q, host, out, scale=scale)
 
 
 @pytest.mark.parametrize("size", [1e-6, 1e-3, 1e3, 1e30])
@@ -440,6 +448,90 @@ def test_long_chunk(pkg):
     gate = torch.randn(q.shape, generator=seqs.gen, device="cuda")
     out, lse, weights = attend(pkg, seqs, q, cu, counts, stats=True, gate=gate)
     check_attention(seqs, q, host, out, lse, weights, gate=gate)
+    out, _, _ = attend(pkg, seqs, q, cu, counts, gate=gate)
+    check_attention(seqs, q, host, out, gate=gate)
+
+
+@pytest.mark.parametrize("kind", ["float16", "bfloat16"])
+@pytest.mark.parametrize("heads", HEADS + [(6, 6, 64), (15, 3, 128), (16, 1, 256), (9, 1, 256)])
+def test_chunks(pkg, heads, kind):
+    """128-row tiles: rows that fill tiles exactly and not, key blocks full and not, tiles cut between CTAs, beside
+    sequences of a few rows and of none."""
+    lens = [64, 65, 128, 1, 200, 3000, 17, 129, 0]
+    counts = [64, 33, 128, 1, 17, 300, 0, 2, 0]
+    seqs = Sequences(pkg, lens, heads, seed=28)
+    q, cu, host = seqs.queries(counts, getattr(torch, kind), pad=5)
+    gate = torch.randn(q.shape, generator=seqs.gen, device="cuda")
+    out, _, _ = attend(pkg, seqs, q, cu, counts)
+    check_attention(seqs, q, host, out)
+    assert (out[host[-1]:] == 77).all()
+    out, _, _ = attend(pkg, seqs, q, cu, counts, gate=gate)
+    check_attention(seqs, q, host, out, gate=gate)
+    again, _, _ = attend(pkg, seqs, q, cu, counts, gate=gate)
+    assert torch.equal(out, again)
+    seqs.cache.check()
+
+
+def test_chunk_values_that_grow(pkg):
+    """V's groups grow by powers of ten along a sequence, each at its own pace, and logits too: what a chunk has
+    summed is brought to the new power or maximum."""
+    heads = (8, 1, 256)
+    seqs = Sequences(pkg, [1500], heads, seed=29)
+    n = seqs.lens[0]
+    at = torch.arange(n, device="cuda")[:, None, None]
+    pace = torch.tensor([0.0, 0.004, 0.008, -0.006], device="cuda").repeat_interleave(64)
+    v = torch.randn(n, 1, 256, generator=seqs.gen, device="cuda") * 10 ** (at * pace - 3)
+    k = torch.randn(n, 1, 256, generator=seqs.gen, device="cuda") * (0.02 + at / 500)
+    seqs.cache.append(None, k, v, None, seqs.slots(0, 0, n), None)
+    (seqs.k[0], seqs.most[0]), seqs.v[0] = quantised(k), quantised(v)[0]
+    q, cu, host = seqs.queries([40], torch.bfloat16)
+    out, _, _ = attend(pkg, seqs, q, cu, [40])
+    ref, _, _, ds = U.attention(q, seqs.k[0], seqs.v[0], seqs.most[0], 1 / 16)
+    ds = ds * (1 + 2.0 ** 12 / 256)
+    for g in range(4):  # each group by its own size
+        part = slice(64 * g, 64 * g + 64)
+        vmax = seqs.v[0][..., part].abs().max().item()
+        d = (out[..., part].double() - ref[..., part]).abs()
+        assert (d <= 2.0 ** -8 * ref[..., part].abs() + (3 * 2.0 ** -11 + 2 * ds[..., None] + 2.0 ** -17) * vmax).all(), g
+
+
+def test_chunk_nan_reaches_only_the_rows_that_see_it(pkg):
+    """NaN keys and values inside a chunk: rows before them are untouched; a value's NaN stays in its group of dims."""
+    heads = (8, 1, 128)
+    seqs = Sequences(pkg, [100], heads, seed=33)
+    q, cu, host = seqs.queries([60], torch.float16)
+    good, _, _ = attend(pkg, seqs, q, cu, [60])
+    k, v = read(seqs.cache, seqs.slots(0, 0, 100))
+    bad_v = v[70:71].clone()
+    bad_v[..., 64:] = math.nan
+    seqs.cache.append(None, k[70:71].contiguous(), bad_v, None, seqs.slots(0, 70, 71), None)
+    out, _, _ = attend(pkg, seqs, q, cu, [60])
+    assert torch.equal(out[:30], good[:30]) and torch.equal(out[30:, :, :64], good[30:, :, :64])
+    assert torch.isnan(out[30:, :, 64:]).all()
+    seqs.cache.append(None, torch.full_like(k[:1], math.inf), v[90:91].contiguous(), None, seqs.slots(0, 90, 91), None)
+    out, _, _ = attend(pkg, seqs, q, cu, [60])
+    assert torch.equal(out[:30], good[:30]) and torch.equal(out[30:50, :, :64], good[30:50, :, :64])
+    assert torch.isnan(out[50:]).all()
+
+
+def test_chunk_queries_of_any_size(pkg):
+    heads = (8, 1, 128)
+    seqs = Sequences(pkg, [100], heads, seed=34)
+    q, cu, host = seqs.queries([20], torch.bfloat16)
+    q[0] *= 1e30
+    q[1] = 0
+    q[2] *= 1e-30
+    out, _, _ = attend(pkg, seqs, q, cu, [20], scale=1e-6)
+    assert torch.isfinite(out).all()
+    ref, _, _, ds = U.attention(q, seqs.k[0], seqs.v[0], seqs.most[0], 1e-6)
+    vmax, ds = seqs.v[0].abs().max(), ds * (1 + 2.0 ** 12 / 128)
+    tol = 2.0 ** -8 * ref.abs() + (3 * 2.0 ** -11 + 2 * ds[..., None] + 2.0 ** -17) * vmax
+    assert ((out.double() - ref).abs()[1:] <= tol[1:]).all()
+    q[5, 3, 7], q[9, 0, 0] = math.nan, math.inf
+    bad, _, _ = attend(pkg, seqs, q, cu, [20], scale=1e-6)
+    assert torch.isnan(bad[5, 3]).all() and torch.isnan(bad[9, 0]).all()
+    bad[5, 3], bad[9, 0] = out[5, 3], out[9, 0]
+    assert torch.equal(bad, out)
 
 
 def test_captured_and_replayed(pkg):

@@ -9,7 +9,7 @@
 //   O[128 x D] += P V     P in TMEM, V^T in shared memory, O in TMEM (D columns)
 // so each MMA reads only its B operand from shared memory. Warp roles:
 //   0-3   softmax: one thread per row; running maximum and sum in registers
-//   4-11  dequantisation: nibbles -> fp16 operands in the 128B-swizzled layout
+//   4-7   dequantisation of K, 8-11 of V: nibbles -> fp16 operands in the 128B-swizzled layout
 //   12    MMA issue    13, 14  bulk copies of the pages' K and V parts
 // The nibbles of the page layout come out as the operands' element pairs: two
 // dims of a K row, two keys of a V^T row. Masked, a pair is an fp16 subnormal
@@ -34,10 +34,11 @@ extern std::atomic<uint64_t> g_kernel_launches;
 namespace {
 
 constexpr int kRows = 128, kKeys = 64, kBlockPages = kKeys / kPageTokens;
-constexpr int kSoftWarps = 4, kDeqWarps = 8, kMmaWarp = 12, kLoadK = 13, kLoadV = 14;
+constexpr int kSoftWarps = 4, kDeqWarps = 4, kMmaWarp = 12, kLoadK = 13, kLoadV = 14;
 constexpr int kThreads = 16 * 32;  // the last warp only completes its warpgroup
 constexpr int kSoftRegs = 152, kOtherRegs = 120;  // of 512 x 128 registers at launch: 128 x (152 + 3 x 120)
 constexpr int kRaw = 3;         // raw page stages, K and V each
+constexpr int kSets = 2;        // sets of steps and biases, K and V each
 constexpr int kUnitBlocks = 4;  // what a unit costs beside its blocks, in blocks
 constexpr int kMinBlocks = 8;   // shortest range
 constexpr int kGroupsMax = 512;
@@ -87,17 +88,21 @@ template <int D>
 struct Smem {
   static constexpr int kHalf = 8 * D;  // nibbles of K or V of a page and head
   alignas(1024) uint8_t k[2][kKeys * D * 2];  // [stage][chunk of 64 dims][key][128 B]
-  alignas(1024) uint8_t v[kKeys * D * 2];     // [dim][64 keys]
+  alignas(1024) uint8_t v[2][kKeys * D * 2];  // [stage][dim][64 keys]
   alignas(16) uint8_t kraw[kRaw][kBlockPages][kHalf + D];  // nibbles, then pairs
   alignas(16) uint8_t vraw[kRaw][kBlockPages][kHalf + D];
-  alignas(16) uint32_t kst[2][kKeys][D / 64][4];  // K, by block: step 2^24, step 2^20, bias (each twice, fp16x2)
-  alignas(16) uint32_t vst[D / 64][kKeys / 2][4];  // V: the same for the two keys of a pair
-  int kpow[8];                              // exponent of K's power of two, by block
-  uint32_t vnan[D / 64][2];                 // keys (even, odd of each pair) whose group is NaN
-  int ve[D / 64], ve_was[D / 64];           // the group's power of two for this block and the block before
+  alignas(16) uint32_t kst[kSets][kKeys][D / 64][4];      // K: step 2^24, step 2^20, bias (each twice, fp16x2)
+  alignas(16) uint32_t vst[kSets][D / 64][kKeys / 2][4];  // V: the same for the two keys of a pair
+  // by block: K's power of two, V's of every group and the one before, the keys
+  // (even, odd of each pair) whose group is NaN
+  alignas(8) float2 kinfo[8];               // K's power times 2^-16, and the bits of the pages that are not there
+  alignas(4) uint8_t vflags[8][4];          // by group: 1 the power has moved, 2 it holds a NaN
+  int ve[8][D / 64], ve_was[8][D / 64];
+  uint32_t vnan[8][D / 64][2];
+  int absent_v[8];
   int absent[8];                            // pages of a block that are outside the pool, by block
   uint64_t kraw_full[kRaw], kraw_empty[kRaw], vraw_full[kRaw], vraw_empty[kRaw];
-  uint64_t k_full[2], k_empty[2], v_full, v_empty, s_full, s_empty, p_full[2], p_empty[2], q_full, o_empty;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full, s_empty, p_full[2], p_empty[2], q_full, o_empty;
   uint32_t tmem;
   int abort;
   int scan[16];
@@ -137,18 +142,30 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
-// Exponent above every magnitude a pair (scale, bias) stands for, kNone for zeros.
+// Largest magnitude that a pair (scale, bias) stands for.
+__device__ __forceinline__ float pair_most(uint32_t pair) {
+  return fmaxf(fabsf(kv4_bias(pair)), fabsf(fmaf(15.f, kv4_scale(pair), kv4_bias(pair))));
+}
+// The power of two that operands are divided by. Divided, magnitudes have to stay
+// below 2^-6 (a step is then at most 2^-5 / 15, and 2^24 times that inside fp16);
+// a new power puts the largest below 2^-9.
 constexpr int kNone = -1000;
-__device__ __forceinline__ int pair_top(float scale, float bias) {
-  const float most = fmaxf(fabsf(bias), fabsf(fmaf(15.f, scale, bias)));
-  return most > 0.f ? min(128, int(__float_as_uint(most) >> 23) - 126) : kNone;
-}
-// The power in use after a block whose magnitudes lie below 2^top: divided by it
-// they have to stay below 2^-6 (a step is then at most 2^-5 / 15, and 2^24 times
-// that inside fp16); a new power puts them below 2^-9.
-__device__ __forceinline__ int next_power(int was, int top) {
-  return top == kNone ? was : was == kNone || top - was > -6 ? top + 9 : was;
-}
+struct Power {
+  int e = kNone;
+  float limit = 0.f;  // magnitudes from here on need a larger power
+  float down = 1.f, down2 = 1.f;  // 2^-e, as two factors for the range's ends
+  // raises the power if the warp's largest magnitude asks for it (an infinity's does not count)
+  __device__ __forceinline__ void raise(float most, bool first) {
+    if (first) *this = Power();
+    if (__any_sync(0xffffffffu, most > limit && most < INFINITY)) {
+      const int top = int(__reduce_max_sync(0xffffffffu, most < INFINITY ? __float_as_uint(most) : 0u) >> 23) - 126;
+      e = top + 9;
+      limit = e > 133 ? FLT_MAX : pow2i(e - 6);
+      down = pow2i(-e / 2);
+      down2 = pow2i(-e - (-e / 2));
+    }
+  }
+};
 __device__ __forceinline__ void sts128(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(p)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -175,11 +192,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.k_full[i], kDeqWarps);
       mbar_init(&sm.k_empty[i], 1);
+      mbar_init(&sm.v_full[i], kDeqWarps);
+      mbar_init(&sm.v_empty[i], 1);
       mbar_init(&sm.p_full[i], kSoftWarps);
       mbar_init(&sm.p_empty[i], 1);
     }
-    mbar_init(&sm.v_full, kDeqWarps);
-    mbar_init(&sm.v_empty, 1);
     mbar_init(&sm.s_full, 1);
     mbar_init(&sm.s_empty, kSoftWarps);
     mbar_init(&sm.q_full, kSoftWarps);
@@ -324,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
         if (n >= kRaw && !wait(&empty[st], (n / kRaw - 1) & 1)) return false;
         const uint32_t there = __ballot_sync(0xffffffffu, from != 0);
         if (lane == 0) {
-          if (key) sm.absent[n & 7] = ~there & ((1 << kBlockPages) - 1);
+          (key ? sm.absent : sm.absent_v)[n & 7] = ~there & ((1 << kBlockPages) - 1);
           if (there) mbar_expect_tx(&full[st], __popc(there) * (kHalf + D));
           else mbar_arrive(&full[st]);
         }
@@ -343,17 +360,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
     for (uint32_t i = n > kRaw ? n - kRaw : 0; i < n; ++i) kv4_wait(&full[i % kRaw], i / kRaw & 1, a.cache.status);
   } else if (warp == kMmaWarp) {
     const uint32_t idesc_s = idesc_f16(kKeys), idesc_o = idesc_f16(D);
-    const uint64_t kdesc = smem_desc_sw128(smem_u32(sm.k[0])), vdesc = smem_desc_sw128(smem_u32(sm.v));
+    const uint64_t kdesc = smem_desc_sw128(smem_u32(sm.k[0])), vdesc = smem_desc_sw128(smem_u32(sm.v[0]));
     uint32_t n = 0, units = 0;  // blocks and units done
     auto pv = [&](uint32_t i, bool first) {
-      if (!wait(&sm.v_full, i & 1) || !wait(&sm.p_full[i & 1], i / 2 & 1)) return false;
+      if (!wait(&sm.v_full[i & 1], i / 2 & 1) || !wait(&sm.p_full[i & 1], i / 2 & 1)) return false;
       if (first && units > 0 && !wait(&sm.o_empty, (units - 1) & 1)) return false;
       tc_fence_after();
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < kKeys / 16; ++k)
-          mma_ts(tmem + kTmO, tmem + kTmP + (i & 1) * 32 + k * 8, vdesc + uint64_t(k * 2), idesc_o, !first || k > 0);
-        mma_commit(&sm.v_empty);
+          mma_ts(tmem + kTmO, tmem + kTmP + (i & 1) * 32 + k * 8, vdesc + uint64_t((i & 1) * sizeof(sm.v[0]) / 16 + k * 2), idesc_o, !first || k > 0);
+        mma_commit(&sm.v_empty[i & 1]);
         mma_commit(&sm.p_empty[i & 1]);
       }
       __syncwarp();
@@ -381,124 +398,141 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
       ++units;
       return true;
     });
-  } else if (warp >= kSoftWarps && warp < kMmaWarp) {
-    const int dt = tid - kSoftWarps * 32, dw = dt >> 5;  // thread and warp among the dequantising ones
-    uint32_t nk = 0, nv = 0;
-    // Steps and biases of a block, a warp per group: V's for block nv (warps 0 ..
-    // NG - 1), K's for block nk (the next NG), then a barrier for all.
-    auto scales_v = [&](const Seq& q, int j, bool first) {
-      const int tok = lane * 2 % kPageTokens, page = lane * 2 / kPageTokens;
-      const uint8_t* raw = sm.vraw[nv % kRaw][page] + Smem<D>::kHalf + dw * 4;
-      const bool there = !(sm.absent[nv & 7] >> page & 1);
-      float scale[2], bias[2];
-      bool nan[2];
+  } else if (warp >= kSoftWarps && warp < kSoftWarps + kDeqWarps) {
+    const int dt = tid - kSoftWarps * 32, dw = dt >> 5;
+    uint32_t n = 0;
+    Power power;  // the same in all warps, for the groups' products add up
+    // Steps and biases of block n as fp16 operands, one set ahead of its values: a
+    // warp per group, a lane for keys lane and lane + 32.
+    auto scales = [&](const Seq& q, int j, bool first) {
+      if (!wait(&sm.kraw_full[n % kRaw], n / kRaw & 1)) return false;
+      if (dw < NG) {
+        float most = 0.f;
+        uint32_t own[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t pair = *reinterpret_cast<const uint32_t*>(raw + (tok + i) * NG * 4);
-        if (!there || j * kKeys + lane * 2 + i >= q.len) pair = 0u;
-        nan[i] = isnan(kv4_bias(pair));
-        if (nan[i]) pair = 0u;  // stands as zero here; the rows that see it are made NaN
-        scale[i] = kv4_scale(pair);
-        bias[i] = kv4_bias(pair);
-      }
-      const int top = __reduce_max_sync(0xffffffffu, max(pair_top(scale[0], bias[0]), pair_top(scale[1], bias[1])));
-      const uint32_t na = __ballot_sync(0xffffffffu, nan[0]), nb = __ballot_sync(0xffffffffu, nan[1]);
-      const int was = first ? kNone : sm.ve[dw], e = next_power(was, top);
-      __syncwarp();
-      if (lane == 0) {
-        sm.ve_was[dw] = was;
-        sm.ve[dw] = e;
-        sm.vnan[dw][0] = na;
-        sm.vnan[dw][1] = nb;
-      }
-      const int d = e == kNone ? 0 : -e;
-      const float down = pow2i(d / 2), down2 = pow2i(d - d / 2);
-      const float s0 = scale[0] * down * down2 * 1048576.f, s1 = scale[1] * down * down2 * 1048576.f;
-      *reinterpret_cast<uint4*>(sm.vst[dw][lane]) =
-          make_uint4(pack_f16(s0 * 16.f, s1 * 16.f), pack_f16(s0, s1), pack_f16(bias[0] * down * down2, bias[1] * down * down2), 0u);
-    };
-    int kpow_now = kNone;  // K's power, the same in every warp that computes it
-    auto scales_k = [&](const Seq& q, int j, bool first) {
-      // all groups share K's power (their products add up): every warp finds the largest of them all
-      int top = kNone;
-      float scale[2], bias[2];
+        for (int i = 0; i < 2; ++i) {
+          const int key = lane + 32 * i, page = key / kPageTokens;
+          alignas(16) uint32_t pair[NG];
+          load_words<NG>(pair, sm.kraw[n % kRaw][page] + Smem<D>::kHalf + key % kPageTokens * NG * 4);
+          const bool there = !(sm.absent[n & 7] >> page & 1) && j * kKeys + key < q.len;  // others are masked later
+          own[i] = 0u;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int key = lane + 32 * i, page = key / kPageTokens;
-        alignas(16) uint32_t pair[NG];
-        load_words<NG>(pair, sm.kraw[nk % kRaw][page] + Smem<D>::kHalf + key % kPageTokens * NG * 4);
-        if ((sm.absent[nk & 7] >> page & 1) || j * kKeys + key >= q.len) {
-#pragma unroll
-          for (int g = 0; g < NG; ++g) pair[g] = 0u;  // masked later: any finite value does
-        }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          top = max(top, pair_top(kv4_scale(pair[g]), kv4_bias(pair[g])));
-          if (g == dw - NG) {
-            scale[i] = kv4_scale(pair[g]);
-            bias[i] = kv4_bias(pair[g]);
+          for (int g = 0; g < NG; ++g) {
+            if (there) most = fmaxf(most, pair_most(pair[g]));
+            if (g == dw && there) own[i] = pair[g];
           }
         }
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      kpow_now = next_power(first ? kNone : kpow_now, top);
-      const int d = kpow_now == kNone ? 0 : -kpow_now;
-      const float down = pow2i(d / 2), down2 = pow2i(d - d / 2);
+        power.raise(most, first);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float s = scale[i] * down * down2 * 1048576.f, b = bias[i] * down * down2;
-        *reinterpret_cast<uint4*>(sm.kst[nk & 1][lane + 32 * i][dw - NG]) = make_uint4(pack_f16(s * 16.f, s * 16.f), pack_f16(s, s), pack_f16(b, b), 0u);
+        for (int i = 0; i < 2; ++i) {
+          const float s = kv4_scale(own[i]) * power.down * power.down2 * 1048576.f, b = kv4_bias(own[i]) * power.down * power.down2;
+          *reinterpret_cast<uint4*>(sm.kst[n % kSets][lane + 32 * i][dw]) = make_uint4(pack_f16(s * 16.f, s * 16.f), pack_f16(s, s), pack_f16(b, b), 0u);
+        }
+        if (dt == 0) sm.kinfo[n & 7] = make_float2(power.e == kNone ? 0.f : pow2i(power.e - 16), __int_as_float(sm.absent[n & 7]));
       }
-      if (dw == NG && lane == 0) sm.kpow[nk & 7] = -d;
+      asm volatile("bar.sync 1, %0;" ::"n"(kDeqWarps * 32) : "memory");
+      return true;
     };
-    auto values_k = [&] {
-      if (nk >= 2 && !wait(&sm.k_empty[nk & 1], (nk / 2 - 1) & 1)) return false;
-      const int st = nk % kRaw, key = dt / 4, t = dt % 4, tok = key % kPageTokens;
-      const uint8_t* raw = sm.kraw[st][key / kPageTokens];
-      alignas(16) uint32_t w[LW];
+    auto values = [&] {
+      const int st = n % kRaw;
+      if (n >= 2 && !wait(&sm.k_empty[n & 1], (n / 2 - 1) & 1)) return false;
+      const int t = dt % 4;
+      alignas(16) uint32_t w[2][LW];
 #pragma unroll
-      for (int i = 0; i < LW; i += L::kChunk) {
-        const uint8_t* p = raw + ((i / L::kChunk * kPageTokens + tok) * 4 + t) * L::kChunk * 4;
-        if constexpr (L::kChunk == 4) *reinterpret_cast<uint4*>(&w[i]) = *reinterpret_cast<const uint4*>(p);
-        else *reinterpret_cast<uint2*>(&w[i]) = *reinterpret_cast<const uint2*>(p);
+      for (int h = 0; h < 2; ++h) {
+        const int key = dt / 4 + 32 * h;
+#pragma unroll
+        for (int i = 0; i < LW; i += L::kChunk) {
+          const uint8_t* p = sm.kraw[st][key / kPageTokens] + ((i / L::kChunk * kPageTokens + key % kPageTokens) * 4 + t) * L::kChunk * 4;
+          if constexpr (L::kChunk == 4) *reinterpret_cast<uint4*>(&w[h][i]) = *reinterpret_cast<const uint4*>(p);
+          else *reinterpret_cast<uint2*>(&w[h][i]) = *reinterpret_cast<const uint2*>(p);
+        }
       }
-      uint8_t* dst = sm.k[nk & 1] + key * 128;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const uint4 c = *reinterpret_cast<const uint4*>(sm.kst[nk & 1][key][g]);
+      for (int h = 0; h < 2; ++h) {
+        const int key = dt / 4 + 32 * h;
+        uint8_t* dst = sm.k[n & 1] + key * 128;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int half = h ^ (key & 1);  // odd keys the other half first: no two keys of a store share banks
-          const uint32_t x = half ? w[2 * g + 1] : w[2 * g], y = x >> 8;
-          sts128(dst + g * kKeys * 128 + ((4 * half + t) ^ (key & 7)) * 16, value_low(x, c.x, c.z), value_high(x, c.y, c.z),
-                 value_low(y, c.x, c.z), value_high(y, c.y, c.z));
+        for (int g = 0; g < NG; ++g) {
+          const uint4 c = *reinterpret_cast<const uint4*>(sm.kst[n % kSets][key][g]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int half = i ^ (key & 1);  // odd keys the other half first: no two keys of a store share banks
+            const uint32_t x = half ? w[h][2 * g + 1] : w[h][2 * g], y = x >> 8;
+            sts128(dst + g * kKeys * 128 + ((4 * half + t) ^ (key & 7)) * 16, value_low(x, c.x, c.z), value_high(x, c.y, c.z),
+                   value_low(y, c.x, c.z), value_high(y, c.y, c.z));
+          }
         }
       }
       proxy_fence();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&sm.kraw_empty[st]);
-        mbar_arrive(&sm.k_full[nk & 1]);
+        mbar_arrive(&sm.k_full[n & 1]);
       }
-      ++nk;
+      ++n;
       return true;
     };
-    auto values_v = [&] {
-      const int st = nv % kRaw;
-      if (dw < 2 * NG) {
+    for_units([&](const Cursor&, const Seq& q, int j0, int blocks, bool, int) {
+      if (blocks && !scales(q, j0, true)) return false;
+      for (int j = 0; j < blocks; ++j)
+        if (!values() || (j + 1 < blocks && !scales(q, j0 + j + 1, false))) return false;
+      return true;
+    });
+  } else if (warp >= kSoftWarps + kDeqWarps && warp < kMmaWarp) {
+    const int dt = tid - (kSoftWarps + kDeqWarps) * 32, dw = dt >> 5;
+    uint32_t n = 0;
+    Power power;  // of this warp's group
+    auto scales = [&](const Seq& q, int j, bool first) {  // a warp per group, a lane per pair of keys
+      if (!wait(&sm.vraw_full[n % kRaw], n / kRaw & 1)) return false;
+      if (dw < NG) {
+        const int tok = lane * 2 % kPageTokens, page = lane * 2 / kPageTokens;
+        const uint8_t* raw = sm.vraw[n % kRaw][page] + Smem<D>::kHalf + tok * NG * 4 + dw * 4;
+        uint32_t a0 = *reinterpret_cast<const uint32_t*>(raw), a1 = *reinterpret_cast<const uint32_t*>(raw + NG * 4);
+        const bool there = !(sm.absent_v[n & 7] >> page & 1);
+        if (!there || j * kKeys + lane * 2 >= q.len) a0 = 0u;
+        if (!there || j * kKeys + lane * 2 + 1 >= q.len) a1 = 0u;
+        // a NaN stands as zero in the operand; the rows that see it are made NaN
+        const uint32_t na = __ballot_sync(0xffffffffu, isnan(kv4_bias(a0))), nb = __ballot_sync(0xffffffffu, isnan(kv4_bias(a1)));
+        if (na >> lane & 1) a0 = 0u;
+        if (nb >> lane & 1) a1 = 0u;
+        const int was = first ? kNone : power.e;
+        power.raise(fmaxf(pair_most(a0), pair_most(a1)), first);
+        const float s0 = kv4_scale(a0) * power.down * power.down2 * 1048576.f, s1 = kv4_scale(a1) * power.down * power.down2 * 1048576.f;
+        *reinterpret_cast<uint4*>(sm.vst[n % kSets][dw][lane]) =
+            make_uint4(pack_f16(s0 * 16.f, s1 * 16.f), pack_f16(s0, s1),
+                       pack_f16(kv4_bias(a0) * power.down * power.down2, kv4_bias(a1) * power.down * power.down2), 0u);
+        if (lane == 0) {
+          sm.ve[n & 7][dw] = power.e;
+          sm.ve_was[n & 7][dw] = was;
+          sm.vnan[n & 7][dw][0] = na;
+          sm.vnan[n & 7][dw][1] = nb;
+          sm.vflags[n & 7][dw] = (was != kNone && was != power.e ? 1 : 0) | (na | nb ? 2 : 0);
+        }
+      } else if (lane == 0) {
+        sm.vflags[n & 7][dw] = 0;
+      }
+      asm volatile("bar.sync 2, %0;" ::"n"(kDeqWarps * 32) : "memory");
+      return true;
+    };
+    auto values = [&] {
+      const int st = n % kRaw;
+      if (n >= 2 && !wait(&sm.v_empty[n & 1], (n / 2 - 1) & 1)) return false;
+#pragma unroll 1
+      for (int part = dw; part < 2 * NG; part += kDeqWarps) {
         // Lane = (word of four, octet of keys). A lane takes its octet's four key
         // pairs in an order turned by the octet, so that the loads of a warp touch
         // every bank once; the columns of V^T keep that order (the weights follow).
-        const int ko = lane & 7, slot = (lane >> 3) + 4 * ((dw & 1) ^ (ko >> 2)), seg = dw >> 1;
+        const int ko = lane & 7, slot = (lane >> 3) + 4 * ((part & 1) ^ (ko >> 2)), seg = part >> 1;
         const int group = slot % NG, gr = seg * L::kRows + slot / NG;
         const uint8_t* raw = sm.vraw[st][ko >> 1] + seg * kPageTokens * 32 + slot * 4;
-        uint8_t* dst = sm.v + (64 * group + 8 * gr) * 128;
+        uint8_t* dst = sm.v[n & 1] + (64 * group + 8 * gr) * 128;
         uint32_t r[8][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int pr = (i + ko) & 3, place = 4 * (ko & 1) + pr;
           const uint32_t x = *reinterpret_cast<const uint32_t*>(raw + place * 32), y = *reinterpret_cast<const uint32_t*>(raw + (place + 8) * 32);
-          const uint4 c = *reinterpret_cast<const uint4*>(sm.vst[group][ko * 4 + pr]);
+          const uint4 c = *reinterpret_cast<const uint4*>(sm.vst[n % kSets][group][ko * 4 + pr]);
           const uint32_t lo = __byte_perm(x, y, 0x5410), hi = __byte_perm(x, y, 0x7632), lo8 = lo >> 8, hi8 = hi >> 8;
           r[0][i] = value_low(lo, c.x, c.z);
           r[1][i] = value_high(lo, c.y, c.z);
@@ -516,28 +550,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&sm.vraw_empty[st]);
-        mbar_arrive(&sm.v_full);
+        mbar_arrive(&sm.v_full[n & 1]);
       }
-      ++nv;
+      ++n;
       return true;
     };
-    // One step: V of block jv (if any) and K of block jk (if any). K runs two blocks ahead of V.
-    auto step = [&](const Seq& q, int jv, bool first_v, int jk, bool first_k) {
-      if (jv >= 0) {
-        if (!wait(&sm.vraw_full[nv % kRaw], nv / kRaw & 1)) return false;
-        if (nv >= 1 && !wait(&sm.v_empty, (nv - 1) & 1)) return false;
-      }
-      if (jk >= 0 && !wait(&sm.kraw_full[nk % kRaw], nk / kRaw & 1)) return false;
-      if (jv >= 0 && dw < NG) scales_v(q, jv, first_v);
-      if (jk >= 0 && dw >= NG && dw < 2 * NG) scales_k(q, jk, first_k);
-      asm volatile("bar.sync 1, %0;" ::"n"(kDeqWarps * 32) : "memory");
-      return (jv < 0 || values_v()) && (jk < 0 || values_k());
-    };
     for_units([&](const Cursor&, const Seq& q, int j0, int blocks, bool, int) {
-      for (int j = -2; j < blocks; ++j) {
-        const int jv = j >= 0 ? j0 + j : -1, jk = j + 2 < blocks ? j0 + j + 2 : -1;
-        if ((jv >= 0 || jk >= 0) && !step(q, jv, j == 0, jk, j == -2)) return false;
-      }
+      if (blocks && !scales(q, j0, true)) return false;
+      for (int j = 0; j < blocks; ++j)
+        if (!values() || (j + 1 < blocks && !scales(q, j0 + j + 1, false))) return false;
       return true;
     });
   } else if (warp < kSoftWarps) {
@@ -591,11 +612,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.q_full);
         const float factor = a.scale * 1.4426950408889634f;
-        const float f1 = fine ? factor * pow2i((e - 14) / 2) * pow2i(e - 14 - (e - 14) / 2) : NAN;
+        const float f1 = factor * pow2i((e + 2) / 2) * pow2i(e + 2 - (e + 2) / 2);  // 2^(e - 14), and the 2^16 that K's power lacks
         const int seen = real ? q.len - q.count + token + 1 : INT_MAX;
         const int least = __reduce_min_sync(0xffffffffu, seen);
         uint32_t poison = 0u;  // groups of which the row sees a NaN
-        int ev[NG];            // V's powers
         for (int j = j0; j < j0 + blocks; ++j, ++n) {
           if (!wait(&sm.s_full, n & 1)) return false;
           tc_fence_after();
@@ -609,9 +629,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
             for (int i = 0; i < kKeys / 2; ++i) x[i] = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
           }
           tc_fence_before();
-          const int absent = sm.absent[n & 7];
-          const int ke = sm.kpow[n & 7];
-          float fk = fine ? fmaxf(f1 * pow2i(ke / 2) * pow2i(ke - ke / 2), FLT_MIN) : NAN;  // above zero: a masked -infinity stays one
+          const float2 info = sm.kinfo[n & 7];
+          const int absent = __float_as_int(info.y);
+          float fk = fine ? fmaxf(f1 * info.x, FLT_MIN) : NAN;  // above zero: a masked -infinity stays one
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.s_empty);
           const int key0 = j * kKeys;
@@ -622,10 +642,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
               if (key0 + 2 * i + 1 >= seen || (absent >> (2 * i / kPageTokens) & 1)) x[i].y = -INFINITY;
             }
           }
-          float top = fmaxf(x[0].x, x[0].y);
+          float tops[4];
 #pragma unroll
-          for (int i = 1; i < kKeys / 2; ++i) top = fmaxf(fmaxf(top, x[i].x), x[i].y);
-          top *= fk;
+          for (int i = 0; i < 4; ++i) tops[i] = fmaxf(x[i].x, x[i].y);
+#pragma unroll
+          for (int i = 4; i < kKeys / 2; ++i) tops[i % 4] = fmaxf(fmaxf(tops[i % 4], x[i].x), x[i].y);
+          const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * fk;
           const bool grow = top > m + kLazy;
           float shrink = 1.f;
           if (grow) {
@@ -659,24 +681,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
             }
           }
           l += sum.x + sum.y;
-          // P's buffer is free once the MMAs before the last are done
-          if (n >= 2 && !wait(&sm.p_empty[n & 1], (n / 2 - 1) & 1)) return false;
+          // With V of this block in place the MMAs on the block before the last are done, so P's buffer is free too
+          if (!wait(&sm.v_full[n & 1], n / 2 & 1)) return false;
           tmem_st32(lanes + kTmP + (n & 1) * 32, p);
-          if (!wait(&sm.v_full, n & 1)) return false;
-          bool moved = false;
-          uint32_t nans = 0u;
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            ev[g] = sm.ve[g];
-            moved = moved || (ev[g] != sm.ve_was[g] && sm.ve_was[g] != kNone);
-            nans |= sm.vnan[g][0] | sm.vnan[g][1];
-          }
-          if (nans) {
+          const uint32_t flags = *reinterpret_cast<const uint32_t*>(sm.vflags[n & 7]);
+          const bool moved = flags & 0x01010101u;
+          if (flags & 0x02020202u) {
 #pragma unroll 1
             for (int g = 0; g < NG; ++g)
 #pragma unroll 1
               for (int i = 0; i < kKeys; ++i)
-                if ((sm.vnan[g][i & 1] >> (i / 2) & 1) && key0 + i < seen) poison |= 1u << g;
+                if ((sm.vnan[n & 7][g][i & 1] >> (i / 2) & 1) && key0 + i < seen) poison |= 1u << g;
           }
           if (j > j0 && (moved || __any_sync(0xffffffffu, grow))) {
             // O so far to the new maximum and powers, when the MMAs on it are done
@@ -684,8 +699,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
-              const int was = sm.ve_was[c / 64];
-              const float f = shrink * (was == kNone ? 1.f : pow2i(was - sm.ve[c / 64]));
+              const int was = sm.ve_was[n & 7][c / 64];
+              const float f = shrink * (was == kNone ? 1.f : pow2i(was - sm.ve[n & 7][c / 64]));
               uint32_t v[32];
               tmem_ld32(lanes + kTmO + c, v);
               tmem_wait_ld();
@@ -709,10 +724,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
           uint32_t v[16];
           tmem_ld16(lanes + kTmO + c, v);
           tmem_wait_ld();
-          int e2 = ev[0];
-#pragma unroll
-          for (int g = 1; g < NG; ++g)
-            if (c >= 64 * g) e2 = ev[g];
+          const int e2 = sm.ve[(n - 1) & 7][c / 64];
           float f = pow2i(e2 == kNone ? 0 : e2 / 2) * (whole ? inv : 1.f);
           const float f2 = pow2i(e2 == kNone ? 0 : e2 - e2 / 2);
           if (poison >> (c / 64) & 1) f = NAN;

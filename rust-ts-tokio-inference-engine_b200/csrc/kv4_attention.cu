@@ -685,46 +685,207 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(Kv4AttentionAr
     a.lse[size_t(seq.first + token) * a.cache.Hq + head] = sum == 0.f ? -INFINITY : (M + log2f(sum)) * 0.6931471805599453f;
 }
 
-// Lane's dims lane E .. lane E + E - 1 of K of one cached token.
-template <int D>
-__device__ __forceinline__ void load_key(const uint8_t* block, int tok, int lane, float (&x)[D / 32]) {
-  using L = Kv4Layout<D>;
-  constexpr int E = D / 32;
-  const int w = lane * E / 8;
-  const uint32_t word = *reinterpret_cast<const uint32_t*>(block + L::k_word(tok, w));
-  const uint32_t pair = *reinterpret_cast<const uint32_t*>(block + L::k_meta(tok, w / 8));
+// What every cached key received from the call's query rows, added to what it
+// had: sum over the rows of exp(logit - lse), with the logits multiplied again from
+// the exact nibbles, as in the decode kernel (the K half of the pages is read once
+// more; keeping all logits would take 4 bytes per key and query head). One CTA per
+// (sequence, KV head, 64 pages), eight pages per warp; a key's sum belongs to one
+// warp, rows in order, so there are no atomics.
+constexpr int kWtWarps = 8, kWtPages = 8, kWtTiles = 4;  // pages of a warp; tiles of query rows held at a time
+
+// The query rows of a tile as B fragments (lane = 4 row + t, register j of word
+// i: dims 2 j, 2 j + 1 of the word's eight), 16 threads per row. A row is
+// scaled by a power of two so that its largest value lies in [2^13, 2^14):
+// fp16 and bf16 queries stay exact; the pairs that meet nibbles carrying 2^4
+// are lowered by as much. Beside them: the factor that brings (q . n) 2^-24
+// back to a logit in base 2, the row's sums over the groups in base 2, and how
+// many keys it sees. A row with a value that is not finite gets NaN sums, so
+// its logits are all NaN.
+template <int D, class T>
+__device__ __forceinline__ void load_tile(const Kv4AttentionArgs& a, const Seq& seq, int head0, int r, int G, bool vec,
+                                          int tid, uint32_t (*frag)[32][4], uint32_t (*sums)[kRowsPerTile][4], float* back, int* seen) {
+  constexpr int kPer = D / 128 > 0 ? D / 128 : 1;  // words of a thread
+  const int rr = tid / 16, j = tid % 16, row = r * kRowsPerTile + rr, token = row / G;
+  const bool real = token < seq.count;
+  const T* src = static_cast<const T*>(a.q.data) + (seq.first + token) * a.q.token_stride + (head0 + row % G) * a.q.head_stride;
+  float x[kPer][8], most = 0.f, sum[kPer];
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    x[e] = fmaf(kv4_scale(pair), float((word >> (4 * kv4_k_nibble(lane * E % 8 + e))) & 15u), kv4_bias(pair));
+  for (int k = 0; k < kPer; ++k) {
+    const int w = j + 16 * k;
+    alignas(16) T raw[8] = {};
+    if (real && w < D / 8) {
+      if (vec) {
+        *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(src + 8 * w);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) raw[e] = src[8 * w + e];
+      }
+    }
+    sum[k] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[k][e] = kv4_to_float(raw[e]);
+      sum[k] += x[k][e];
+      // the largest magnitude; a NaN's bits are above every number's
+      most = __uint_as_float(max(__float_as_uint(most), __float_as_uint(x[k][e]) & 0x7FFFFFFFu));
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) most = __uint_as_float(max(__float_as_uint(most), __shfl_xor_sync(0xffffffffu, __float_as_uint(most), o)));
+  const bool fine = __float_as_uint(most) < 0x7F800000u;
+  const int e = most > 0.f && fine ? int(__float_as_uint(most) >> 23) - 126 : 0;  // |row| < 2^e
+  const float up = pow2i((14 - e) / 2), up2 = fine ? pow2i(14 - e - (14 - e) / 2) : 0.f;
+  const float factor = a.scale * 1.4426950408889634f;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int w = j + 16 * k;
+    if (w < D / 8) {
+      uint32_t v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float lift = (i & 1 ? 0.0625f : 1.f) * up2;
+        v[i] = fine ? pack_f16(x[k][2 * i] * up * lift, x[k][2 * i + 1] * up * lift) : 0u;
+      }
+      *reinterpret_cast<uint4*>(frag[2 * (w / 8) + w % 8 / 4][4 * rr + w % 4]) = make_uint4(v[0], v[1], v[2], v[3]);
+      if (w % 8 == 0) {
+        const float total = fine ? sum[k] * factor : NAN;
+        float rest = total;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const uint32_t top = uint32_t(float_to_bf16_bits(rest)) << 16;
+          sums[i][rr][w / 8] = top;
+          rest -= __uint_as_float(top);
+        }
+      }
+    }
+  }
+  if (j >= D / 64 && j < 4) {  // groups this head_dim does not have
+#pragma unroll
+    for (int i = 0; i < 3; ++i) sums[i][rr][j] = 0u;
+  }
+  if (j == 0) {
+    back[rr] = factor * pow2i((e + 10) / 2) * pow2i(e + 10 - (e + 10) / 2);
+    seen[rr] = real ? seq.len - seq.count + token + 1 : INT_MAX;  // rows past the last are not written
+  }
 }
 
-// One CTA per (sequence, KV head, page): what each key received from the
-// sequence's query tokens and the head's group, added to what it had.
+template <int D>
+struct WtSmem {
+  alignas(16) uint32_t q[kWtTiles][Kv4Layout<D>::kLaneWords][32][4];
+  uint32_t sum[kWtTiles][3][kRowsPerTile][4];
+  float back[kWtTiles][kRowsPerTile], lse[kWtTiles][kRowsPerTile];
+  int seen[kWtTiles][kRowsPerTile];
+  float acc[kWtWarps][kWtPages][kPageTokens];
+};
+
 template <int D, class T>
-__global__ void __launch_bounds__(128) kv4_weights_kernel(Kv4AttentionArgs a, const float* __restrict__ lse) {
+__global__ void __launch_bounds__(kWtWarps * 32) kv4_weights_kernel(Kv4AttentionArgs a, int chunks, bool q_vec) {
   pdl_trigger();
-  pdl_wait(lse);
-  constexpr int E = D / 32;
-  const int s = blockIdx.y / a.cache.Hkv, g = blockIdx.y % a.cache.Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int G = a.cache.Hq / a.cache.Hkv;
-  const Seq q = load_seq(a, s, G, false);
-  for (int p = blockIdx.x * kPageTokens + warp; p < min(q.len, (int(blockIdx.x) + 1) * kPageTokens); p += 4) {
-    const size_t at = (size_t(s) * a.cache.Hkv + g) * a.weights_stride + p;
-    float sum = a.weights_in && p < q.len - q.count ? a.weights_in[at] : 0.f;
-    const int64_t page = a.table[s * a.table_stride + p / kPageTokens];
-    if (page >= 0 && uint64_t(page) < a.cache.pages) {
-      float k[E];
-      load_key<D>(a.cache.block(uint64_t(page), g), p % kPageTokens, lane, k);
-      for (int j = max(0, p - (q.len - q.count)); j < q.count; ++j)
-        for (int h = g * G; h < (g + 1) * G; ++h) {
-          const T* x = static_cast<const T*>(a.q.data) + (q.first + j) * a.q.token_stride + h * a.q.head_stride;
-          float dot = 0.f;
-#pragma unroll
-          for (int e = 0; e < E; ++e) dot = fmaf(kv4_to_float(x[lane * E + e]), k[e], dot);
-          sum += __expf(warp_sum(dot) * a.scale - lse[size_t(q.first + j) * a.cache.Hq + h]);
-        }
+  pdl_wait();
+  using L = Kv4Layout<D>;
+  constexpr int NG = L::kGroups, LW = L::kLaneWords;
+  __shared__ WtSmem<D> sm;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, tq = lane & 3;
+  const int Hkv = a.cache.Hkv, G = a.cache.Hq / Hkv;
+  const int chunk = blockIdx.x % chunks, g = blockIdx.x / chunks % Hkv, s = blockIdx.x / chunks / Hkv;
+  const Seq seq = load_seq(a, s, G, false);
+  const int page0 = chunk * kWtWarps * kWtPages, pages = (seq.len + kPageTokens - 1) / kPageTokens;
+  if (page0 >= pages) return;
+  const int mine = min(kWtPages, max(0, (pages - page0 - warp + kWtWarps - 1) / kWtWarps));
+  for (int i = lane; i < kWtPages * kPageTokens; i += 32) (&sm.acc[warp][0][0])[i] = 0.f;
+  const int tiles = (seq.count * G + kRowsPerTile - 1) / kRowsPerTile;
+  for (int r0 = 0; r0 < tiles; r0 += kWtTiles) {
+    const int n_tiles = min(kWtTiles, tiles - r0);
+    __syncthreads();
+    for (int i = tid / 128; i < n_tiles; i += kWtWarps * 32 / 128) {
+      const int r = r0 + i, t16 = tid % 128;
+      load_tile<D, T>(a, seq, g * G, r, G, q_vec, t16, sm.q[i], sm.sum[i], sm.back[i], sm.seen[i]);
+      if (t16 % 16 == 0) {
+        const int row = r * kRowsPerTile + t16 / 16, token = row / G;
+        const bool real = token < seq.count;
+        sm.lse[i][t16 / 16] = real ? a.lse[size_t(seq.first + token) * a.cache.Hq + g * G + row % G] * 1.4426950408889634f : 0.f;
+        if (!real) sm.seen[i][t16 / 16] = 0;
+      }
     }
-    if (lane == 0) a.weights_out[at] = sum;
+    __syncthreads();
+    for (int k = 0; k < mine; ++k) {
+      const int page = page0 + warp + k * kWtWarps;
+      const int64_t id = a.table[s * a.table_stride + page];
+      if (id < 0 || uint64_t(id) >= a.cache.pages) continue;
+      const uint8_t* blk = a.cache.block(uint64_t(id), g);
+      alignas(16) uint32_t w0[LW], w1[LW], km[2][NG];
+#pragma unroll
+      for (int i = 0; i < LW; i += L::kChunk) {
+        const uint8_t* p0 = blk + ((i / L::kChunk * kPageTokens + gr) * 4 + tq) * L::kChunk * 4;
+        const uint8_t* p1 = p0 + 8 * 4 * L::kChunk * 4;
+        if constexpr (L::kChunk == 4) {
+          *reinterpret_cast<uint4*>(&w0[i]) = *reinterpret_cast<const uint4*>(p0);
+          *reinterpret_cast<uint4*>(&w1[i]) = *reinterpret_cast<const uint4*>(p1);
+        } else {
+          *reinterpret_cast<uint2*>(&w0[i]) = *reinterpret_cast<const uint2*>(p0);
+          *reinterpret_cast<uint2*>(&w1[i]) = *reinterpret_cast<const uint2*>(p1);
+        }
+      }
+      load_words<NG>(km[0], blk + L::k_meta(gr, 0));
+      load_words<NG>(km[1], blk + L::k_meta(gr + 8, 0));
+      uint32_t m0 = km[0][0], m1 = km[1][0];  // the pair of group tq % NG
+#pragma unroll
+      for (int i = 1; i < NG; ++i)
+        if (tq % NG == i) m0 = km[0][i], m1 = km[1][i];
+      float sum[2] = {0.f, 0.f};
+      for (int i = 0; i < n_tiles; ++i) {
+        const int seen0 = sm.seen[i][2 * tq], seen1 = sm.seen[i][2 * tq + 1];
+        float acc[NG][4], part[4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint4 q[NG];
+#pragma unroll
+          for (int e = 0; e < NG; ++e) q[e] = *reinterpret_cast<const uint4*>(sm.q[i][2 * e + j][lane]);
+#pragma unroll
+          for (int e = 0; e < NG; ++e) {
+            const uint32_t x = w0[2 * e + j], y = w1[2 * e + j];
+            if (j == 0) mma_f16_first(acc[e], x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q[e].x, q[e].y);
+            else mma_f16(acc[e], x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q[e].x, q[e].y);
+          }
+#pragma unroll
+          for (int e = 0; e < NG; ++e) {
+            const uint32_t x = w0[2 * e + j] >> 8, y = w1[2 * e + j] >> 8;
+            mma_f16(acc[e], x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q[e].z, q[e].w);
+          }
+        }
+        mma_bf16_first(part, m0, m1, m0, m1, sm.sum[i][0][gr][tq], sm.sum[i][1][gr][tq]);
+        mma_bf16(part, m0, m1, m0, m1, sm.sum[i][2][gr][tq], 0u);
+        const float f0 = sm.back[i][2 * tq], f1 = sm.back[i][2 * tq + 1], l0 = sm.lse[i][2 * tq], l1 = sm.lse[i][2 * tq + 1];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x0 = kv4_scale(km[c][0]) * acc[0][2 * c], x1 = kv4_scale(km[c][0]) * acc[0][2 * c + 1];
+#pragma unroll
+          for (int e = 1; e < NG; ++e) {
+            x0 = fmaf(kv4_scale(km[c][e]), acc[e][2 * c], x0);
+            x1 = fmaf(kv4_scale(km[c][e]), acc[e][2 * c + 1], x1);
+          }
+          const int key = page * kPageTokens + gr + 8 * c;
+          const float p0 = exp2_fast(fmaf(x0, f0, part[2 * c]) - l0), p1 = exp2_fast(fmaf(x1, f1, part[2 * c + 1]) - l1);
+          sum[c] += (key < seen0 ? p0 : 0.f) + (key < seen1 ? p1 : 0.f);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], 1);
+        sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], 2);
+        if (tq == 0) sm.acc[warp][k][gr + 8 * c] += sum[c];
+      }
+    }
+  }
+  __syncwarp();
+  const size_t row = (size_t(s) * Hkv + g) * a.weights_stride;
+  for (int i = lane; i < mine * kPageTokens; i += 32) {
+    const int key = (page0 + warp + i / kPageTokens * kWtWarps) * kPageTokens + i % kPageTokens;
+    if (key >= seq.len) continue;
+    const float old = a.weights_in && key < seq.len - seq.count ? a.weights_in[row + key] : 0.f;
+    a.weights_out[row + key] = old + sm.acc[warp][i / kPageTokens][i % kPageTokens];
   }
 }
 
@@ -734,9 +895,11 @@ size_t decode_workspace(int Hq, int Hkv, int D, size_t n_seq, size_t tokens, int
 }
 
 // Rows of a sequence up to which it runs here when neither lse nor weights are
-// asked for: two tiles, which this kernel reads the pages for twice; from three
-// on the 128-row tiles of kv4_chunk_kernel are faster.
-constexpr int kChunkRows = 16;
+// asked for: five tiles, for each of which this kernel reads the pages again. From
+// six on the 128-row tiles of kv4_chunk_kernel are faster: 64 sequences of 4096
+// keys at head_dim 256 take 137 us here with 32 rows and 169 there, 194 and 171
+// with 48.
+constexpr int kChunkRows = 40;
 
 template <int D, class T>
 void attend(const Kv4AttentionArgs& a, cudaStream_t s) {
@@ -763,8 +926,9 @@ void attend(const Kv4AttentionArgs& a, cudaStream_t s) {
   g_kernel_launches.fetch_add(2, std::memory_order_relaxed);
   if (chunks) launch_kv4_chunk(b, static_cast<uint8_t*>(a.workspace) + decode_workspace(a.cache.Hq, a.cache.Hkv, D, a.n_seq, a.tokens, a.sm_count), s);
   if (a.weights_out) {
-    launch_pdl(kv4_weights_kernel<D, T>, dim3(unsigned(a.table_stride), a.n_seq * a.cache.Hkv), 128, 0, s, b,
-               static_cast<const float*>(b.lse));
+    const int64_t chunks = (a.table_stride + kWtWarps * kWtPages - 1) / (kWtWarps * kWtPages);
+    if (chunks * a.n_seq * a.cache.Hkv > INT32_MAX) throw std::invalid_argument("kv4 attention: n_seq x kv_heads x pages beyond 2^31; split the call");
+    launch_pdl(kv4_weights_kernel<D, T>, unsigned(chunks * a.n_seq * a.cache.Hkv), kWtWarps * 32, 0, s, b, int(chunks), q_vec);
     g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
   }
 }

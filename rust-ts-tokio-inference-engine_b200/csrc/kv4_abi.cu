@@ -163,7 +163,7 @@ int rs_qwen_kv4_read(const rs_qwen_kv4_cache* cache, size_t tokens, const int64_
     if (!tokens) return;
     need(slots && aligned(slots, 8), "kv4 read: slots missing or not 8-byte aligned");
     need(k && v && aligned(k, 16) && aligned(v, 16), "kv4 read: outputs missing or not 16-byte aligned");
-    need(tokens * size_t(c.Hkv) * size_t(c.D / 8) <= size_t(INT32_MAX) * 256, "kv4 read: too many tokens");
+    need(tokens * size_t(c.Hkv) * size_t(c.D / 4) <= size_t(INT32_MAX) * 256, "kv4 read: too many tokens");
     OnDevice on(cache->device);
     launch_kv4_read(c, int64_t(tokens), slots, dtype, k, v, static_cast<cudaStream_t>(stream));
   });
@@ -245,8 +245,8 @@ int rs_qwen_kv4_evict(const rs_qwen_kv4_cache* cache, const rs_qwen_kv4_evict_ar
     need(args->weights_stride >= 1, "kv4 evict: weights_stride must be positive");
     need(!args->weights_out || args->weights_out_stride >= args->keep, "kv4 evict: weights_out_stride must cover keep");
     need(args->weights_out != args->weights, "kv4 evict: weights_out must not be weights");
-    need(args->n_seq * uint64_t(cache->kv_heads) * uint64_t(args->keep) <= uint64_t(INT32_MAX) * 8,
-         "kv4 evict: too many kept keys");
+    need(args->keep <= INT32_MAX / 32 && args->n_seq * uint64_t(cache->kv_heads) * ((uint64_t(args->keep) * (cache->head_dim / 16 + 2) + 255) / 256) <=
+             uint64_t(INT32_MAX), "kv4 evict: too many kept keys");
     a.n_seq = int(args->n_seq);
     a.kv_lens = args->kv_lens;
     a.src_table = args->src_table;

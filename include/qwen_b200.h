@@ -331,6 +331,36 @@ int rs_qwen_device_ep_connect(void* session, const uint8_t* handles, size_t hand
 int rs_qwen_device_synthetic_state(void* session, size_t position, uint64_t seed, StateId* out,
                                    char* error, size_t capacity);
 
+/* NEW (no reference counterpart): the session keeps its attention keys and
+ * values in 4 bits (the groups, rounding and layout of the rs_qwen_kv4 section
+ * below) instead of bf16: 3.56 times the pages in the same byte budget, and as
+ * much less to read per step. Call it before any admission and before
+ * mtp_attach; the MTP draft head keeps bf16 pages. Steps, blocks, verify, forks,
+ * synthetic states and snapshots then work on the 4-bit pages (a snapshot holds
+ * the values as read back). head_dim must be 64, 128 or 256 with at most 16 query
+ * heads per KV head.
+ * track = 1 also keeps, per version, layer, KV head and key, the attention weight
+ * that the key has received so far (kv_heads x context x 4 bytes per layer and
+ * slot, taken from the byte budget), which rs_qwen_device_kv4_evict ranks by; a
+ * tracked session refuses mtp_verify_accept, whose rejected tokens would count,
+ * and its long prefills run the kernel that keeps softmax statistics. */
+int rs_qwen_device_kv4(void* session, int track, char* error, size_t capacity);
+/* For each of n_seq versions a new version at the same position that holds only
+ * `keep` keys per layer and KV head (all, if it has no more): the last `recent`
+ * and, of the others, those with the largest accumulated weight (the earlier one
+ * on ties). Later tokens keep their true positions. The new versions have pages,
+ * weights and a copy of the DeltaNet state of their own; the old ones stay until
+ * they are released. Snapshots of versions with evicted keys are refused. */
+int rs_qwen_device_kv4_evict(void* session, size_t n_seq, const StateId* ids, size_t keep, size_t recent,
+                             StateId* outs, char* error, size_t capacity);
+
+/* What a version's cache holds in attention layer `layer` (0 is the first one):
+ * *held keys, read back as k, v [kv_heads][count][head_dim] and the weights they
+ * have received, [kv_heads][count], in host memory; count must be *held. With
+ * k, v and weights NULL only *held is written; k and v, or weights, may be NULL. */
+int rs_qwen_device_kv4_read(void* session, const StateId* id, size_t layer, float* k, float* v, float* weights,
+                            size_t count, size_t* held, char* error, size_t capacity);
+
 /* NEW diagnostic (no reference counterpart; mirrors the role of the
  * reference's routing probe, native/operator_probe.inc:19-23): when enabled,
  * each step keeps its top-k expert ids; rs_qwen_device_debug_routing copies
@@ -395,8 +425,9 @@ int rs_qwen_project_noalloc(void* session, int which, int layer, const void* x_d
 /* ---- 4-bit paged KV cache (no reference counterpart) ----
  *
  * The attention cache of one layer in 4 bits, on memory the caller owns, for
- * servers whose contexts do not fit the sessions' bf16 pages. Keys and values
- * are quantised per (token, KV head) in groups of 64 dims:
+ * servers whose contexts do not fit the sessions' bf16 pages (rs_qwen_device_kv4
+ * is a session on such pages). Keys and values are quantised per (token, KV
+ * head) in groups of 64 dims:
  *   scale = bf16((max - min) / 15), bias = bf16(min),
  *   n = clamp(rint((x - bias) / scale), 0, 15), value = scale * n + bias
  * (n = 0 where scale is 0; a group that holds an infinity or NaN reads back as
@@ -477,7 +508,13 @@ int rs_qwen_kv4_read(const rs_qwen_kv4_cache* cache, size_t tokens, const int64_
  * weights_out (or NULL): [n_seq][kv_heads][weights_stride], for each key of a
  * sequence weights_in (NULL: zero) plus the softmax weight it received from all
  * the call's query rows of its KV head; the newest n keys start from zero.
- * weights_in may be weights_out. Columns from kv_lens[s] on are not written. */
+ * weights_in may be weights_out. Columns from kv_lens[s] on are not written.
+ * Sums are fp32. Without lse and weights, sequences that feed more than 40 query
+ * rows per KV head (max_count x q_heads / kv_heads) round keys, values and
+ * softmax weights to fp16 (2^-11 each) on their way to the tensor cores; the
+ * others, and every sequence when lse or weights are asked for, use the stored
+ * nibbles exactly. A call's n_seq x kv_heads x query tiles x pages must stay
+ * below 2^31 (an error otherwise: split the call). */
 typedef struct {
   rs_qwen_kv4_rows q, gate, out;
   uint32_t dtype, reserved;

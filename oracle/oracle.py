@@ -85,6 +85,7 @@ def lib():
         L.orc_last_error.restype = C.c_char_p
         L.orc_set_routing_slack.argtypes = [C.c_double]
         L.orc_set_emulation.argtypes = [C.c_int]
+        L.orc_set_cached_kv.argtypes = [F]
         L.orc_state_count.restype = SZ
         L.orc_state_count.argtypes = [C.POINTER(RsQwenConfig)]
         L.orc_model_create.restype = P
@@ -194,10 +195,21 @@ class Model:
         return out
 
     def forward(self, tokens, offset: int, old_state=None, hidden: bool = False,
-                forced_routing=None):
-        """Returns (logits [count, vocab] f64, new_state f32, hidden or None, routing)."""
+                forced_routing=None, cached_kv=None):
+        """Returns (logits [count, vocab] f64, new_state f32, hidden or None, routing). cached_kv [attention layers,
+        2, kv_heads, count, head_dim]: the keys and values that a 4-bit cache holds for these tokens; attention
+        reads them instead of its own, which they must be near."""
         c = self.cfg
         tok = np.ascontiguousarray(tokens, np.uint32)
+        if cached_kv is not None:
+            held = np.ascontiguousarray(cached_kv, np.float32)
+            if held.shape != (c.layers // c.interval, 2, c.kv_heads, len(tok), c.head_dim):
+                raise ValueError("cached_kv shape")
+            lib().orc_set_cached_kv(_p(held, C.c_float))
+            try:
+                return self.forward(tokens, offset, old_state, hidden, forced_routing)
+            finally:
+                lib().orc_set_cached_kv(None)
         n = self.state_count()
         new = np.zeros(n, np.float32)
         old = _f32(old_state) if old_state is not None else np.zeros(1, np.float32)

@@ -53,6 +53,13 @@ double g_routing_slack = 2e-3;
 //   256: the 16-bit type is IEEE half instead of bfloat16
 int g_emulate = 0;
 
+// Keys and values of the fed tokens that a quantising cache holds, [attention
+// layers][K, V][kv][tokens][d]: attention then reads these, each checked to be
+// within `g_kv_slack` of a 4-bit step of the oracle's own. Null: its own.
+const float* g_forced_kv = nullptr;
+size_t g_forced_kv_layer = 0;
+double g_kv_slack = 5e-2;
+
 double round16(double v) {
   if (g_emulate & 256) return double(float(_Float16(float(v))));
   return double(synth::bf16_to_float(synth::bf16_rne(float(v))));
@@ -451,6 +458,20 @@ struct Forward {
           Kc[(g * ctx + offset + t) * d + i] = (g_emulate & 4) ? round16(tmp[i]) : tmp[i];
           Vc[(g * ctx + offset + t) * d + i] = (g_emulate & 4) ? round16(v[(t * Hk + g) * d + i]) : v[(t * Hk + g) * d + i];
         }
+        if (g_forced_kv)
+          for (int sel = 0; sel < 2; ++sel) {
+            double* own = (sel ? Vc : Kc) + (g * ctx + offset + t) * d;
+            const float* held = g_forced_kv + (((g_forced_kv_layer * 2 + sel) * Hk + g) * T + t) * d;
+            for (size_t i0 = 0; i0 < d; i0 += 64) {
+              const double range = *std::max_element(own + i0, own + i0 + 64) - *std::min_element(own + i0, own + i0 + 64);
+              // half a step; sqrt 2 of it where a key was rotated after it was stored
+              for (size_t i = i0; i < i0 + 64; ++i) {
+                if (!(std::abs(held[i] - own[i]) <= (std::sqrt(2.) / 30 + g_kv_slack) * range + g_kv_slack * std::abs(own[i])))
+                  throw std::invalid_argument("oracle: the cached key or value is not near the oracle's");
+                own[i] = double(held[i]);
+              }
+            }
+          }
       }
     // attention_reference.h:8-21, bottom-right causal window.
     std::vector<double> o(T * Hq * d);
@@ -581,6 +602,9 @@ void orc_set_routing_slack(double slack) { g_routing_slack = slack; }
 // Error-analysis knobs (bits documented at g_emulate); 0 restores exact FP64.
 void orc_set_emulation(int bits) { g_emulate = bits; }
 
+// Cached keys and values of the next forward's tokens (see g_forced_kv); null: off.
+void orc_set_cached_kv(const float* kv) { g_forced_kv = kv; }
+
 size_t orc_state_count(const rs_qwen_config* c) { return state_count(*c); }
 
 // Build a lazily generated synthetic model (same tensors and bytes as
@@ -666,6 +690,7 @@ int orc_forward(void* model, const uint32_t* tokens, size_t count, size_t offset
     f.forced_count = forced_count;
     f.routed_out = routed;
     size_t H = c.hidden, T = count, ctx = c.context, d = c.head_dim, Hk = c.kv_heads;
+    g_forced_kv_layer = 0;
     size_t convn = size_t(c.conv - 1) * f.cd, sn = size_t(c.value_heads) * c.value_dim * c.key_dim;
     std::vector<double> x(T * H), h(T * H), r(T * H);
     f.embed(tokens, T, x.data());
@@ -681,6 +706,7 @@ int orc_forward(void* model, const uint32_t* tokens, size_t count, size_t offset
         }
         rd += 2 * K.size();
         f.attention(p, h.data(), T, offset, K.data(), V.data(), ctx, r.data());
+        ++g_forced_kv_layer;
         for (size_t i = 0; i < K.size(); ++i) new_state[wr + i] = float(K[i]);
         for (size_t i = 0; i < V.size(); ++i) new_state[wr + K.size() + i] = float(V[i]);
         wr += 2 * K.size();

@@ -146,6 +146,9 @@ SIGNATURES = {
     "rs_qwen_device_mtp_verify_accept": (C.c_int, [_P, _SZ, _SIDP, _U32P, _U32P, _U32P, _SZ, _U32P, _SZ,
                                                    C.c_uint32, _SIDP, _U32P, _U32P, _U32P, _ERR, _SZ]),
     "rs_qwen_device_synthetic_state": (C.c_int, [_P, _SZ, C.c_uint64, _SIDP, _ERR, _SZ]),
+    "rs_qwen_device_kv4": (C.c_int, [_P, C.c_int, _ERR, _SZ]),
+    "rs_qwen_device_kv4_read": (C.c_int, [_P, _SIDP, _SZ, _F32P, _F32P, _F32P, _SZ, C.POINTER(_SZ), _ERR, _SZ]),
+    "rs_qwen_device_kv4_evict": (C.c_int, [_P, _SZ, _SIDP, _SZ, _SZ, _SIDP, _ERR, _SZ]),
     "rs_qwen_device_set_capture": (C.c_int, [_P, C.c_int, _ERR, _SZ]),
     "rs_qwen_device_set_profile": (C.c_int, [_P, C.c_int, _ERR, _SZ]),
     "rs_qwen_ep_unique_id": (C.c_int, [C.c_void_p, _SZ, _ERR, _SZ]),
@@ -472,6 +475,30 @@ class DeviceSession:
         out = StateId()
         _call("rs_qwen_device_synthetic_state", self.h, position, seed, C.byref(out))
         return out
+
+    def kv4(self, track: bool = False):
+        """Attention pages in 4 bits (rs_qwen_device_kv4); before any admission and mtp_attach."""
+        _call("rs_qwen_device_kv4", self.h, int(track))
+        return self
+
+    def kv4_read(self, sid: StateId, layer: int, weights: bool = False):
+        """Keys, values [kv_heads, held, head_dim] and weights [kv_heads, held] (or None) that a version's cache
+        holds in attention layer `layer` (rs_qwen_device_kv4_read)."""
+        held = C.c_size_t()
+        _call("rs_qwen_device_kv4_read", self.h, C.byref(sid), layer, None, None, None, 0, C.byref(held))
+        shape = (self.cfg.kv_heads, held.value, self.cfg.head_dim)
+        k, v = np.zeros(shape, np.float32), np.zeros(shape, np.float32)
+        w = np.zeros(shape[:2], np.float32) if weights else None
+        _call("rs_qwen_device_kv4_read", self.h, C.byref(sid), layer, _ptr(k, C.c_float), _ptr(v, C.c_float),
+              _ptr(w, C.c_float), held.value, C.byref(held))
+        return k, v, w
+
+    def kv4_evict(self, sids, keep: int, recent: int):
+        """New versions that keep `keep` keys per layer and KV head (rs_qwen_device_kv4_evict)."""
+        n = len(sids)
+        ids, outs = (StateId * n)(*sids), (StateId * n)()
+        _call("rs_qwen_device_kv4_evict", self.h, n, ids, keep, recent, outs)
+        return list(outs)
 
     def set_capture(self, routing: bool):
         _call("rs_qwen_device_set_capture", self.h, int(routing))

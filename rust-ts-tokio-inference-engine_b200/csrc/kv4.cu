@@ -360,9 +360,10 @@ __global__ void __launch_bounds__(kSelThreads) kv4_select_kernel(Kv4EvictArgs a)
     if (tid == 0) kv4_flag(a.cache.status, kErrBounds);
     len = int(min(max(int64_t(len), int64_t(0)), most));
   }
-  const float* w = a.weights + (size_t(s) * a.cache.Hkv + h) * a.weights_stride;
+  const int from = a.weights_rows ? a.weights_rows[s] : s, to = a.weights_out_rows ? a.weights_out_rows[s] : s;
+  const float* w = a.weights + (size_t(from) * a.cache.Hkv + h) * a.weights_stride;
   int32_t* kept = a.kept + (size_t(s) * a.cache.Hkv + h) * a.keep;
-  float* wo = a.weights_out ? a.weights_out + (size_t(s) * a.cache.Hkv + h) * a.weights_out_stride : nullptr;
+  float* wo = a.weights_out ? a.weights_out + (size_t(to) * a.cache.Hkv + h) * a.weights_out_stride : nullptr;
   const int n_new = min(len, a.keep);
   if (tid == 0 && h == 0) a.new_lens[s] = n_new;
   for (int j = n_new + tid; j < a.keep; j += kSelThreads) {

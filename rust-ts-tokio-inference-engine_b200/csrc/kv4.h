@@ -108,6 +108,8 @@ struct Kv4AttentionArgs {
   const float* weights_in = nullptr;    // [n_seq][Hkv][weights_stride]
   float* weights_out = nullptr;
   int64_t weights_stride = 0;
+  const int32_t* weights_in_rows = nullptr;   // row of each sequence (null: its own index; negative: none, zeros)
+  const int32_t* weights_out_rows = nullptr;
   void* workspace = nullptr;
   size_t workspace_bytes = 0;
   int sm_count = 0;
@@ -128,6 +130,8 @@ struct Kv4EvictArgs {
   int64_t src_stride = 0, dst_stride = 0;
   const float* weights = nullptr;  // [n_seq][Hkv][weights_stride]
   int64_t weights_stride = 0;
+  const int32_t* weights_rows = nullptr;  // row of each sequence (null: its own index)
+  const int32_t* weights_out_rows = nullptr;
   int keep = 0, recent = 0;
   int32_t* kept = nullptr;  // [n_seq][Hkv][keep]
   int32_t* new_lens = nullptr;
@@ -135,6 +139,25 @@ struct Kv4EvictArgs {
   int64_t weights_out_stride = 0;
 };
 void launch_kv4_evict(const Kv4EvictArgs& a, cudaStream_t s);
+
+// ---- a session's 4-bit pages (kv4_session.cu) ----
+struct SeqDesc;
+// A step's tables, in batch order.
+struct Kv4Tables {
+  int32_t* kv_lens = nullptr;   // [n_seq] cache length after the step
+  int32_t* table = nullptr;     // [n_seq][stride]
+  int32_t* parents = nullptr;   // [n_seq] state slots
+  int32_t* children = nullptr;
+  int64_t* slots = nullptr;     // [tokens]
+  int stride = 0;
+};
+// dropped: evicted keys of each sequence, null = none
+void launch_kv4_tables(const SeqDesc* descs, int n_seq, const int32_t* dropped, const int32_t* block_table, int stride,
+                       const int32_t* cu_seqlens, const Kv4Tables& t, cudaStream_t s);
+void launch_kv4_cow(uint8_t* pool, int layers, size_t layer_bytes, size_t page_bytes, const SeqDesc* descs, int n_seq,
+                    const int32_t* new_pages, cudaStream_t s);
+void launch_kv4_synth(float* k, float* v, int first, int count, int Hkv, int D, int ctx, int layer, uint64_t seed,
+                      cudaStream_t s);
 
 // ---- element access by type ----
 template <class T>

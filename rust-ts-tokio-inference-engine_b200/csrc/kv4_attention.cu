@@ -880,12 +880,14 @@ __global__ void __launch_bounds__(kWtWarps * 32) kv4_weights_kernel(Kv4Attention
     }
   }
   __syncwarp();
-  const size_t row = (size_t(s) * Hkv + g) * a.weights_stride;
+  const int from = a.weights_in_rows ? a.weights_in_rows[s] : s, to = a.weights_out_rows ? a.weights_out_rows[s] : s;
+  const float* in = a.weights_in && from >= 0 ? a.weights_in + (size_t(from) * Hkv + g) * a.weights_stride : nullptr;
+  float* out = a.weights_out + (size_t(to) * Hkv + g) * a.weights_stride;
   for (int i = lane; i < mine * kPageTokens; i += 32) {
     const int key = (page0 + warp + i / kPageTokens * kWtWarps) * kPageTokens + i % kPageTokens;
     if (key >= seq.len) continue;
-    const float old = a.weights_in && key < seq.len - seq.count ? a.weights_in[row + key] : 0.f;
-    a.weights_out[row + key] = old + sm.acc[warp][i / kPageTokens][i % kPageTokens];
+    const float old = in && key < seq.len - seq.count ? in[key] : 0.f;
+    out[key] = old + sm.acc[warp][i / kPageTokens][i % kPageTokens];
   }
 }
 

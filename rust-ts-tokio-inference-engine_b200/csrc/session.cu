@@ -22,6 +22,7 @@
 #include <nccl.h>
 
 #include "kernels.h"
+#include "kv4.h"
 #include "noalloc.h"
 #include "qgemm_tc.h"
 #include "state_table.h"
@@ -150,6 +151,7 @@ struct PinBuf {
 struct Version {
   std::vector<int32_t> pages;  // KV pages covering [0, position)
   uint32_t hidden_rows = 0;    // post-norm hidden rows kept (hidden_* calls)
+  int dropped = 0;             // evicted keys: the pages cover [0, position - dropped)
 };
 
 // MTP draft version (native/qwen_mtp.inc): KV of the MTP attention layer for
@@ -221,6 +223,17 @@ struct Session {
   size_t mpage_bytes = 0;
   size_t draft_residents() const { return drafts ? drafts->residents() : 0; }
   uint64_t draft_bytes() const { return drafts ? drafts->bytes() : 0; }
+  // 4-bit pages in place of the bf16 ones (rs_qwen_device_kv4): [layer][page][KV
+  // head][block], and with tracking each version's accumulated attention weights
+  // [layer][slot][KV head][context]
+  bool kv4_on = false, kv4_track = false;
+  DevBuf<uint8_t> kv4_mem, kv4_ws;
+  DevBuf<float> kv4_weights;
+  DevBuf<int32_t> kv4_lens, kv4_table, kv4_parents, kv4_children, kv4_dropped, kv4_kept, kv4_new_lens;
+  DevBuf<int64_t> kv4_slots;
+  size_t kv4_page = 0, kv4_weight_bytes = 0;  // of one layer's page; of a version's weights
+  int kv4_max_count = 0;
+  bool kv4_any_dropped = false;
   int attn_split_pages = 16, attn_n_items = 0, attn_splits = 1, pf_n_blocks = 0, n_merge = 0;
   DevBuf<gemm_in_t> hb, hb2, act, xperm, hb_out;  // projection inputs (fp16)
   int sm_count = 148;
@@ -376,7 +389,7 @@ struct Session {
   void set_device() const { QWEN_CUDA(cudaSetDevice(device)); }
 
   uint64_t version_bytes(size_t n_pages, size_t hidden_rows) const {
-    return gdn_slot_bytes + n_pages * page_bytes + hidden_rows * size_t(d.H) * 4;
+    return gdn_slot_bytes + kv4_weight_bytes + n_pages * page_bytes + hidden_rows * size_t(d.H) * 4;
   }
 
   void unref_pages(const std::vector<int32_t>& pages) {
@@ -518,10 +531,298 @@ struct Session {
     kv.Hkv = d.Hkv;
     kv.D = d.D;
     for (int l = 0; l < d.n_attn && budget_pages > 0; ++l) kv_maps.push_back(make_kv_map(kv, l));
-    free_pages.resize(budget_pages);
-    for (size_t i = 0; i < budget_pages; ++i) free_pages[i] = int32_t(budget_pages - 1 - i);
-    page_ref.assign(budget_pages, 0);
-    page_filled.assign(budget_pages, 0);
+    reset_pages(budget_pages);
+  }
+
+  void reset_pages(size_t n) {
+    free_pages.resize(n);
+    for (size_t i = 0; i < n; ++i) free_pages[i] = int32_t(n - 1 - i);
+    page_ref.assign(n, 0);
+    page_filled.assign(n, 0);
+  }
+
+  // ------------------------------------------------------------ 4-bit pages --
+  // rs_qwen_device_kv4: the page pool in 4 bits, in the same byte budget.
+  void kv4_enable(bool track) {
+    if (kv4_on) throw std::invalid_argument("4-bit pages already in use");
+    if (d.n_attn == 0) throw std::invalid_argument("4-bit pages need an attention layer");
+    if (table->residents()) throw std::invalid_argument("4-bit pages must precede admission");
+    if (mtp_on) throw std::invalid_argument("4-bit pages must precede MTP attach");
+    if ((d.D != 64 && d.D != 128 && d.D != 256) || d.Hq % d.Hkv || d.Hq / d.Hkv > 16)
+      throw std::invalid_argument("4-bit pages: head_dim 64, 128 or 256 and at most 16 query heads per KV head");
+    const size_t page = size_t(d.Hkv) * kv4_block_bytes(d.D), layers_page = page * d.n_attn;
+    const size_t weight_elems = track ? size_t(d.n_attn) * d.Hkv * d.ctx : 0;
+    const uint64_t fixed = uint64_t(slots) * (gdn_slot_bytes + weight_elems * 4);
+    if (limit <= fixed || (limit - fixed) / layers_page == 0)
+      throw std::invalid_argument("state byte budget smaller than the DeltaNet pool and the tracked weights");
+    set_device();
+    QWEN_CUDA(cudaStreamSynchronize(stream));
+    reset_pages(0);
+    kv_maps.clear();
+    kv_mem.release();
+    kv.base = nullptr;
+    kv.layers = kv.n_pages = 0;
+    kv4_on = true;
+    kv4_page = page;
+    page_bytes = layers_page;
+    if (track) {
+      kv4_weights.ensure(weight_elems * slots);
+      kv4_weight_bytes = weight_elems * 4;
+      kv4_track = true;
+    }
+    size_t free_b = 0, total_b = 0;
+    QWEN_CUDA(cudaMemGetInfo(&free_b, &total_b));
+    const size_t headroom = size_t(2) << 30;
+    const size_t pages = std::min({size_t((limit - fixed) / page_bytes),
+                                   free_b > headroom ? (free_b - headroom) / page_bytes : size_t(0),
+                                   size_t(INT32_MAX / kPageTokens)});
+    if (pages == 0) throw std::runtime_error("no device memory left for KV pages");
+    kv4_mem.ensure(pages * page_bytes);
+    kv4_lens.ensure(max_seqs);
+    kv4_new_lens.ensure(max_seqs);
+    kv4_parents.ensure(max_seqs);
+    kv4_children.ensure(max_seqs);
+    kv4_dropped.ensure(max_seqs);
+    kv4_slots.ensure(max_tokens);
+    kv.n_pages = int(pages);
+    reset_pages(pages);
+  }
+
+  Kv4View kv4_view(int layer) const {
+    Kv4View v;
+    v.pool = kv4_mem.p + size_t(layer) * kv.n_pages * kv4_page;
+    v.pages = uint64_t(kv.n_pages);
+    v.Hq = d.Hq;
+    v.Hkv = d.Hkv;
+    v.D = d.D;
+    v.status = err.p;
+    return v;
+  }
+  // Row of slot 0 in one layer's accumulated weights.
+  float* kv4_layer_weights(int layer) const { return kv4_weights.p + size_t(layer) * slots * d.Hkv * d.ctx; }
+
+  // Norm, rotation, 4-bit append and attention of one layer's projection: fp16
+  // queries (|q| is bounded by the norm: sqrt(head_dim) times its gain) and rows out.
+  void kv4_attention(const LayerDev& ly, int proj_w, int splits, size_t split_stride, int n, int T, cudaStream_t s) {
+    const int64_t ld = proj_w;
+    Kv4AppendArgs a;
+    a.cache = kv4_view(ly.type_index);
+    a.q = {partial.p, ld, 2 * d.D};
+    a.gate = partial.p + d.D;
+    a.k = {partial.p + size_t(d.Hq) * 2 * d.D, ld, d.D};
+    a.v = {partial.p + size_t(d.Hq) * 2 * d.D + size_t(d.Hkv) * d.D, ld, d.D};
+    a.tokens = T;
+    a.splits = splits;
+    a.split_stride = split_stride;
+    a.q_norm = ly.q_norm;
+    a.k_norm = ly.k_norm;
+    a.eps = d.eps;
+    a.theta = double(d.theta);
+    a.rope = d.rope;
+    a.positions = token_pos.p;
+    a.slots = kv4_slots.p;
+    a.q_out = q.p;
+    a.gate_out = gate.p;
+    launch_kv4_append(a, s);
+    const int64_t row = int64_t(d.Hq) * d.D;
+    Kv4AttentionArgs t;
+    t.cache = a.cache;
+    t.q = {q.p, row, d.D};
+    t.gate = {gate.p, row, d.D};
+    t.out = hb2.p;
+    t.out_token_stride = row;
+    t.out_head_stride = d.D;
+    t.n_seq = n;
+    t.tokens = T;
+    t.max_count = kv4_max_count;
+    t.cu_seqlens = cu_seqlens.p;
+    t.kv_lens = kv4_lens.p;
+    t.table = kv4_table.p;
+    t.table_stride = bt_stride;
+    t.scale = 1.f / std::sqrt(float(d.D));
+    if (kv4_track) {
+      t.weights_in = t.weights_out = kv4_layer_weights(ly.type_index);
+      t.weights_stride = d.ctx;
+      t.weights_in_rows = kv4_parents.p;
+      t.weights_out_rows = kv4_children.p;
+    }
+    t.workspace = kv4_ws.p;
+    t.workspace_bytes = kv4_workspace_bytes(d.Hq, d.Hkv, d.D, size_t(n), size_t(T), sm_count);
+    t.sm_count = sm_count;
+    launch_kv4_attention(t, s);
+  }
+
+  // rs_qwen_device_kv4_evict: for each version a child at the same position that
+  // keeps the last `recent` keys and the most attended of the others, per layer and
+  // KV head, on pages of its own. The DeltaNet state is copied.
+  void kv4_evict(size_t n, const StateId* ids, size_t keep_in, size_t recent_in, StateId* outs) {
+    if (!kv4_track) throw std::invalid_argument("eviction needs 4-bit pages with tracked weights");
+    if (!n || n > size_t(max_seqs)) throw std::invalid_argument("eviction batch");
+    if (!keep_in || keep_in > size_t(d.ctx) || recent_in > keep_in)
+      throw std::invalid_argument("eviction: keep must be 1 to the context, recent at most keep");
+    set_device();
+    std::vector<const Version*> par(n);
+    std::vector<int32_t> held(n), from(n), to(n);
+    int most = 0;
+    for (size_t i = 0; i < n; ++i) {
+      par[i] = &table->get(ids[i]);
+      held[i] = int32_t(ids[i].position) - par[i]->dropped;
+      from[i] = int32_t(ids[i].slot);
+      most = std::max(most, held[i]);
+    }
+    if (table->residents() + draft_residents() + n > slots) throw std::runtime_error("combined resident budget exhausted");
+    const int keep = std::min(int(keep_in), most), recent = std::min(int(recent_in), keep);
+    const size_t stride = size_t(bt_stride);
+    std::vector<int32_t> tables(2 * n * stride, 0);
+    std::vector<Version> made(n);
+    std::vector<StateId> reserved;
+    try {
+      for (size_t i = 0; i < n; ++i) {
+        const int left = std::min(held[i], keep);
+        const size_t pages = size_t(left + kPageTokens - 1) / kPageTokens;
+        if (pages > free_pages.size()) throw std::runtime_error("KV page pool exhausted");
+        made[i].dropped = int(ids[i].position) - left;
+        for (size_t j = 0; j < pages; ++j) {
+          const int32_t p = free_pages.back();
+          free_pages.pop_back();
+          page_ref[p] = 1;
+          page_filled[p] = uint8_t(std::min<size_t>(kPageTokens, size_t(left) - j * kPageTokens));
+          made[i].pages.push_back(p);
+        }
+        reserved.push_back(table->reserve(ids[i].position, version_bytes(pages, 0)));
+        to[i] = int32_t(reserved[i].slot);
+        std::copy(par[i]->pages.begin(), par[i]->pages.end(), tables.begin() + i * stride);
+        std::copy(made[i].pages.begin(), made[i].pages.end(), tables.begin() + (n + i) * stride);
+      }
+      cudaStream_t s = stream;
+      kv4_table.ensure_grow(2 * n * stride, s);
+      kv4_kept.ensure_grow(n * d.Hkv * keep, s);
+      auto up = [&](int32_t* dst, const std::vector<int32_t>& v) {
+        QWEN_CUDA(cudaMemcpyAsync(dst, v.data(), v.size() * 4, cudaMemcpyHostToDevice, s));
+      };
+      up(kv4_table.p, tables);
+      up(kv4_lens.p, held);
+      up(kv4_parents.p, from);
+      up(kv4_children.p, to);
+      QWEN_CUDA(cudaMemsetAsync(err.p, 0, 4, s));
+      const size_t se = gdn.state_elems * d.n_gdn, ce = gdn.conv_elems * d.n_gdn;
+      for (size_t i = 0; i < n; ++i) {
+        up(block_table.p + size_t(to[i]) * stride, made[i].pages);
+        if (se) QWEN_CUDA(cudaMemcpyAsync(gdn.state + to[i] * se, gdn.state + from[i] * se, se * 4, cudaMemcpyDeviceToDevice, s));
+        if (ce) QWEN_CUDA(cudaMemcpyAsync(gdn.conv + to[i] * ce, gdn.conv + from[i] * ce, ce * 4, cudaMemcpyDeviceToDevice, s));
+      }
+      for (int l = 0; l < d.n_attn; ++l) {
+        Kv4EvictArgs a;
+        a.cache = kv4_view(l);
+        a.n_seq = int(n);
+        a.kv_lens = kv4_lens.p;
+        a.src_table = kv4_table.p;
+        a.dst_table = kv4_table.p + n * stride;
+        a.src_stride = a.dst_stride = bt_stride;
+        a.weights = kv4_layer_weights(l);
+        a.weights_out = kv4_layer_weights(l);
+        a.weights_stride = a.weights_out_stride = d.ctx;
+        a.weights_rows = kv4_parents.p;
+        a.weights_out_rows = kv4_children.p;
+        a.keep = keep;
+        a.recent = recent;
+        a.kept = kv4_kept.p;
+        a.new_lens = kv4_new_lens.p;
+        launch_kv4_evict(a, s);
+      }
+      uint32_t h_err = 0;
+      QWEN_CUDA(cudaMemcpyAsync(&h_err, err.p, 4, cudaMemcpyDeviceToHost, s));
+      QWEN_CUDA(cudaStreamSynchronize(s));
+      if (h_err) throw std::runtime_error("eviction error flag " + std::to_string(h_err));
+    } catch (...) {
+      cudaStreamSynchronize(stream);
+      for (auto& v : made) unref_pages(v.pages);
+      for (auto& id : reserved) {
+        try {
+          table->rollback(id);
+        } catch (...) {
+        }
+      }
+      throw;
+    }
+    for (size_t i = 0; i < n; ++i) {
+      table->publish(reserved[i], std::move(made[i]));
+      outs[i] = reserved[i];
+    }
+  }
+
+  // Synthetic keys and values of [0, position) of every layer into a version's
+  // pages: the bf16 session's values, in 4 bits.
+  void kv4_synthetic(const std::vector<int32_t>& pages, size_t slot, int position, uint64_t seed) {
+    const int step = std::min(position, 2048);
+    const size_t row = size_t(d.Hkv) * d.D;
+    DevBuf<float> k, v;
+    DevBuf<int64_t> where;
+    k.ensure(step * row);
+    v.ensure(step * row);
+    where.ensure(position);
+    std::vector<int64_t> at(position);
+    for (int i = 0; i < position; ++i) at[i] = int64_t(pages[i / kPageTokens]) * kPageTokens + i % kPageTokens;
+    QWEN_CUDA(cudaMemcpyAsync(where.p, at.data(), at.size() * 8, cudaMemcpyHostToDevice, stream));
+    for (int l = 0; l < d.n_attn; ++l)
+      for (int first = 0; first < position; first += step) {
+        Kv4AppendArgs a;
+        a.cache = kv4_view(l);
+        a.tokens = std::min(step, position - first);
+        a.k = {k.p, int64_t(row), d.D};
+        a.v = {v.p, int64_t(row), d.D};
+        a.slots = where.p + first;
+        launch_kv4_synth(k.p, v.p, first, a.tokens, d.Hkv, d.D, d.ctx, l, seed, stream);
+        launch_kv4_append(a, stream);
+      }
+    if (kv4_track)  // nothing has attended to them yet
+      QWEN_CUDA(cudaMemset2DAsync(kv4_weights.p + slot * size_t(d.Hkv) * d.ctx, slots * d.Hkv * size_t(d.ctx) * 4, 0,
+                                  size_t(d.Hkv) * d.ctx * 4, d.n_attn, stream));
+    QWEN_CUDA(cudaStreamSynchronize(stream));
+  }
+
+  // The first n cached keys and values of one layer and version as [kv][stride][d].
+  void kv4_values(const Version& ver, int layer, size_t n, size_t stride, float* k, float* v) {
+    const size_t row = size_t(d.Hkv) * d.D, step = std::min<size_t>(n, 2048);
+    DevBuf<float> kv_dev;
+    DevBuf<int64_t> where;
+    kv_dev.ensure(2 * step * row);
+    where.ensure(step);
+    std::vector<float> host(2 * step * row);
+    std::vector<int64_t> at(step);
+    for (size_t first = 0; first < n; first += step) {
+      const size_t m = std::min(step, n - first);
+      for (size_t i = 0; i < m; ++i)
+        at[i] = int64_t(ver.pages[(first + i) / kPageTokens]) * kPageTokens + int64_t((first + i) % kPageTokens);
+      QWEN_CUDA(cudaMemcpyAsync(where.p, at.data(), m * 8, cudaMemcpyHostToDevice, stream));
+      launch_kv4_read(kv4_view(layer), int64_t(m), where.p, kKv4F32, kv_dev.p, kv_dev.p + step * row, stream);
+      QWEN_CUDA(cudaMemcpyAsync(host.data(), kv_dev.p, host.size() * 4, cudaMemcpyDeviceToHost, stream));
+      QWEN_CUDA(cudaStreamSynchronize(stream));
+      for (int sel = 0; sel < 2; ++sel)
+        for (size_t i = 0; i < m; ++i)
+          for (int g = 0; g < d.Hkv; ++g)
+            std::memcpy((sel ? v : k) + (size_t(g) * stride + first + i) * d.D,
+                        host.data() + sel * step * row + i * row + size_t(g) * d.D, size_t(d.D) * 4);
+    }
+  }
+
+  // rs_qwen_device_kv4_read
+  void kv4_read(const StateId& id, size_t layer, float* k, float* v, float* weights, size_t count, size_t* held) {
+    if (!kv4_on) throw std::invalid_argument("the session's pages are not 4-bit");
+    const Version& ver = table->get(id);
+    if (layer >= size_t(d.n_attn)) throw std::invalid_argument("attention layer out of range");
+    const size_t n = size_t(id.position) - size_t(ver.dropped);
+    *held = n;
+    if (!k && !v && !weights) return;
+    if (count != n) throw std::invalid_argument("kv4 read capacity");
+    if (!k != !v) throw std::invalid_argument("keys and values go together");
+    if (weights && !kv4_track) throw std::invalid_argument("the session does not track attention weights");
+    set_device();
+    QWEN_CUDA(cudaStreamSynchronize(stream));
+    if (k) kv4_values(ver, int(layer), n, n, k, v);
+    if (weights)
+      QWEN_CUDA(cudaMemcpy2D(weights, n * 4, kv4_layer_weights(int(layer)) + id.slot * size_t(d.Hkv) * d.ctx,
+                             size_t(d.ctx) * 4, n * 4, d.Hkv, cudaMemcpyDeviceToHost));
   }
 
   // ------------------------------------------------------------ the step --
@@ -608,7 +909,11 @@ struct Session {
     std::vector<int4> pf_blocks;
     std::vector<int32_t> merge_tokens;
     attn_n_items = pf_n_blocks = 0;
-    if (d.n_attn > 0) {
+    if (kv4_on) {
+      if (vin && kv4_track) throw std::invalid_argument("speculative verify on a session that tracks attention weights");
+      kv4_max_count = 0;
+      for (const auto& s : seqs) kv4_max_count = std::max(kv4_max_count, int(s.count));
+    } else if (d.n_attn > 0) {
       const int G = d.Hq / d.Hkv;
       const bool pf_ok = G >= 1 && G <= 16 && 16 % G == 0;
       const int QB = pf_ok ? kAttnPrefillWarps * (16 / G) : 0;
@@ -714,6 +1019,7 @@ struct Session {
     std::vector<StateId> reserved;
     std::vector<int32_t> deferred_free;
     std::vector<int> tok_off(n + 1, 0);
+    std::vector<int32_t> dropped(n, 0);  // evicted keys (4-bit pages)
     std::vector<std::vector<StateId>> cands(vin ? n : 0);  // verify: per token's candidate version
     std::vector<int32_t> cand_host;
     // On failure every page reference taken for a child is dropped (shared
@@ -740,7 +1046,9 @@ struct Session {
         sd.count = int32_t(s.count);
         sd.parent = s.parent ? int32_t(s.parent->slot) : -1;
         sd.cow_src = -1;
-        const int pos = int(s.position), cnt = int(s.count);
+        // pos: place in the cache, behind the keys that the prefix still holds
+        dropped[i] = par[i] ? par[i]->dropped : 0;
+        const int pos = int(s.position) - dropped[i], cnt = int(s.count);
         const int n_prefix = (pos + kPageTokens - 1) / kPageTokens;
         const int n_total = (pos + cnt + kPageTokens - 1) / kPageTokens;
         if (par[i] && int(par[i]->pages.size()) != n_prefix) throw std::runtime_error("parent page list inconsistent");
@@ -839,6 +1147,11 @@ struct Session {
           QWEN_CUDA(cudaMemcpyAsync(eos_dev.p, vin->eos, vin->n_eos * 4, cudaMemcpyHostToDevice, stream));
       }
       QWEN_CUDA(cudaMemsetAsync(err.p, 0, 4, stream));
+      kv4_any_dropped = std::any_of(dropped.begin(), dropped.end(), [](int32_t x) { return x > 0; });
+      if (kv4_any_dropped) {
+        QWEN_CUDA(cudaMemcpyAsync(kv4_dropped.p, dropped.data(), dropped.size() * 4, cudaMemcpyHostToDevice, stream));
+        uploads += dropped.size() * 4;
+      }
       if (!items.empty()) {
         attn_items.ensure_grow(items.size(), stream);
         QWEN_CUDA(cudaMemcpyAsync(attn_items.p, hi, items.size() * 8, cudaMemcpyHostToDevice, stream));
@@ -983,6 +1296,7 @@ struct Session {
       Version v;
       v.pages = std::move(child_pages[i]);
       v.hidden_rows = keep_hidden ? seqs[i].count : 0;
+      v.dropped = dropped[i];
       table->publish(reserved[i], std::move(v));
       outs[i] = reserved[i];
     }
@@ -1002,10 +1316,18 @@ struct Session {
     Packed pk{cu_seqlens.p, token_seq.p, token_pos.p, slot_mapping.p, out_token.p};
     stage(0);  // Embedding (packing + embedding)
     launch_pack(descs.p, n, new_pages.p, block_table.p, bt_stride, pk, s);
-    if (d.n_attn > 0) launch_cow(kv, descs.p, n, new_pages.p, s);
+    if (kv4_on) {
+      launch_kv4_cow(kv4_mem.p, d.n_attn, size_t(kv.n_pages) * kv4_page, kv4_page, descs.p, n, new_pages.p, s);
+      kv4_table.ensure_grow(size_t(n) * bt_stride, s);
+      kv4_ws.ensure_grow(kv4_workspace_bytes(d.Hq, d.Hkv, d.D, size_t(n), size_t(T), sm_count), s);
+      launch_kv4_tables(descs.p, n, kv4_any_dropped ? kv4_dropped.p : nullptr, block_table.p, bt_stride, cu_seqlens.p,
+                        {kv4_lens.p, kv4_table.p, kv4_parents.p, kv4_children.p, kv4_slots.p, bt_stride}, s);
+    } else if (d.n_attn > 0) {
+      launch_cow(kv, descs.p, n, new_pages.p, s);
+    }
     launch_embed_norm(m.embed, tokens.p, T, m.layers[0].in_norm, d.eps, x.p, hb.p, s);
     const int slots_per_tok = d.top + 1, A = T * slots_per_tok;
-    if (d.n_attn > 0) attn_ws.ensure_grow(size_t(pf_n_blocks ? n_merge : T) * d.Hq * attn_splits * (d.D + 2), s);
+    if (d.n_attn > 0 && !kv4_on) attn_ws.ensure_grow(size_t(pf_n_blocks ? n_merge : T) * d.Hq * attn_splits * (d.D + 2), s);
     if (capture_routing) {
       capture.ensure(size_t(d.L) * A);
       cap_logits.ensure(size_t(d.L) * T * (d.E + 1));
@@ -1028,16 +1350,20 @@ struct Session {
         stage(5);  // RecurrentOutput
       } else {
         stage(7);  // AttentionReduction (q/k norm, RoPE, KV append, paged attention)
-        launch_attn_prep(d, ly, partial.p, proj_w, ps, proj_stride, token_pos.p, slot_mapping.p, T, kv,
-                         ly.type_index, q.p, gate.p, s);
-        launch_attn_decode(kv_maps[ly.type_index], d, q.p, token_seq.p, token_pos.p,
-                           pf_n_blocks ? merge_dev.p : nullptr, descs.p, block_table.p,
-                           bt_stride, attn_items.p, attn_n_items, attn_split_pages, attn_ws.p, attn_splits, err.p,
-                           s);
-        launch_attn_prefill(kv_maps[ly.type_index], d, q.p, token_pos.p, descs.p, block_table.p, bt_stride,
-                            pf_dev.p, pf_n_blocks, gate.p, hb2.p, err.p, s);
-        launch_attention_merge(d, attn_ws.p, gate.p, token_pos.p, pf_n_blocks ? merge_dev.p : nullptr,
-                               pf_n_blocks ? n_merge : T, attn_split_pages, attn_splits, hb2.p, s);
+        if (kv4_on) {
+          kv4_attention(ly, proj_w, ps, proj_stride, n, T, s);
+        } else {
+          launch_attn_prep(d, ly, partial.p, proj_w, ps, proj_stride, token_pos.p, slot_mapping.p, T, kv,
+                           ly.type_index, q.p, gate.p, s);
+          launch_attn_decode(kv_maps[ly.type_index], d, q.p, token_seq.p, token_pos.p,
+                             pf_n_blocks ? merge_dev.p : nullptr, descs.p, block_table.p,
+                             bt_stride, attn_items.p, attn_n_items, attn_split_pages, attn_ws.p, attn_splits, err.p,
+                             s);
+          launch_attn_prefill(kv_maps[ly.type_index], d, q.p, token_pos.p, descs.p, block_table.p, bt_stride,
+                              pf_dev.p, pf_n_blocks, gate.p, hb2.p, err.p, s);
+          launch_attention_merge(d, attn_ws.p, gate.p, token_pos.p, pf_n_blocks ? merge_dev.p : nullptr,
+                                 pf_n_blocks ? n_merge : T, attn_split_pages, attn_splits, hb2.p, s);
+        }
         stage(8);  // AttentionOutput
       }
       const size_t out_stride = size_t(T) * d.H;
@@ -1083,6 +1409,7 @@ struct Session {
   void export_snapshot(const StateId& id, float* output, size_t count) {
     const Version& v = table->get(id);
     if (count != d.state_count()) throw std::invalid_argument("snapshot capacity");
+    if (v.dropped) throw std::invalid_argument("snapshot of a version with evicted keys");
     set_device();
     QWEN_CUDA(cudaStreamSynchronize(stream));
     size_t off = 0;
@@ -1101,7 +1428,8 @@ struct Session {
       } else {
         const size_t per = size_t(d.Hkv) * d.ctx * d.D;
         std::fill(output + off, output + off + 2 * per, 0.f);
-        for (size_t pi = 0; pi < v.pages.size(); ++pi) {
+        if (kv4_on) kv4_values(v, ly.type_index, pos, d.ctx, output + off, output + off + per);
+        for (size_t pi = 0; !kv4_on && pi < v.pages.size(); ++pi) {
           QWEN_CUDA(cudaMemcpy(page.data(), kv.page(ly.type_index, v.pages[pi]), page.size() * 2,
                                cudaMemcpyDeviceToHost));
           for (int kvsel = 0; kvsel < 2; ++kvsel)
@@ -2075,11 +2403,7 @@ int rs_qwen_device_drain(void* session, uint64_t* invalidated, char* error, size
     s->set_device();
     QWEN_CUDA(cudaStreamSynchronize(s->stream));
     s->table->clear();
-    const size_t np = s->page_ref.size();
-    s->free_pages.resize(np);
-    for (size_t i = 0; i < np; ++i) s->free_pages[i] = int32_t(np - 1 - i);
-    std::fill(s->page_ref.begin(), s->page_ref.end(), 0);
-    std::fill(s->page_filled.begin(), s->page_filled.end(), 0);
+    s->reset_pages(s->page_ref.size());
     if (s->table->residents() || s->table->bytes()) throw std::runtime_error("device drain residual");
     if (s->mtp_on) {  // draft versions too (native/qwen_device.inc:65 drains both tables)
       *invalidated += s->drafts->residents();
@@ -2428,6 +2752,7 @@ int rs_qwen_device_synthetic_state(void* session, size_t position, uint64_t seed
       launch_synth_state(s->kv, s->new_pages.p, n_pages, int(position), s->d.ctx, s->gdn, int(id.slot), s->d,
                          seed, s->stream);
       QWEN_CUDA(cudaGetLastError());
+      if (s->kv4_on) s->kv4_synthetic(v.pages, id.slot, int(position), seed);
       QWEN_CUDA(cudaStreamSynchronize(s->stream));
     } catch (...) {
       s->unref_pages(v.pages);
@@ -2436,6 +2761,29 @@ int rs_qwen_device_synthetic_state(void* session, size_t position, uint64_t seed
     }
     s->table->publish(id, std::move(v));
     *out = id;
+  });
+}
+
+int rs_qwen_device_kv4(void* session, int track, char* error, size_t capacity) {
+  return checked(error, capacity, [&] {
+    if (track != 0 && track != 1) throw std::invalid_argument("kv4 tracking must be 0 or 1");
+    S(session)->kv4_enable(track != 0);
+  });
+}
+
+int rs_qwen_device_kv4_read(void* session, const StateId* id, size_t layer, float* k, float* v, float* weights,
+                            size_t count, size_t* held, char* error, size_t capacity) {
+  return checked(error, capacity, [&] {
+    if (!id || !held) throw std::invalid_argument("kv4 read descriptor");
+    S(session)->kv4_read(*id, layer, k, v, weights, count, held);
+  });
+}
+
+int rs_qwen_device_kv4_evict(void* session, size_t n_seq, const StateId* ids, size_t keep, size_t recent,
+                             StateId* outs, char* error, size_t capacity) {
+  return checked(error, capacity, [&] {
+    if (!ids || !outs) throw std::invalid_argument("eviction descriptor");
+    S(session)->kv4_evict(n_seq, ids, keep, recent, outs);
   });
 }
 

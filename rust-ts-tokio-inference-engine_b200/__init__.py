@@ -11,6 +11,7 @@ machine without a B200.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -565,7 +566,19 @@ class DeviceSession:
 # ---- 4-bit paged KV cache ----
 
 KV4_PAGE = 16  # tokens per page
-_KV4_TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+# Kv4AppendArgs and Kv4AttentionArgs in one call
+_KV4_APPEND = struct.Struct("=" + 3 * "Qqq" + "IIQQQQQQffii")
+_KV4_ATTENTION = struct.Struct("=" + 3 * "Qqq" + "IIQQQQQQqf4xQQQqQQ")
+
+
+def _pack(kind, layout, *values):
+    try:
+        return kind.from_buffer_copy(layout.pack(*values))
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"kv4: argument out of range: {e}") from None
+
+
+assert _KV4_APPEND.size == C.sizeof(Kv4AppendArgs) and _KV4_ATTENTION.size == C.sizeof(Kv4AttentionArgs)
 
 
 def kv4_page_bytes(kv_heads: int, head_dim: int) -> int:
@@ -588,17 +601,21 @@ class Kv4Cache:
     met a page id, slot or length out of range (see check())."""
 
     def __init__(self, pool, q_heads: int, kv_heads: int, head_dim: int, status=None):
+        import torch
+        self._current_stream = torch.cuda.current_stream
+        self._f32, self._i32, self._i64, self._u8 = torch.float32, torch.int32, torch.int64, torch.uint8
+        self._types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
         page = kv4_page_bytes(kv_heads, head_dim)
-        if str(pool.dtype) != "torch.uint8" or not pool.is_contiguous() or not pool.is_cuda:
+        if pool.dtype != torch.uint8 or not pool.is_contiguous() or not pool.is_cuda:
             raise ValueError("kv4: the pool is a contiguous uint8 CUDA tensor")
         if pool.numel() < page or pool.numel() % page:
             raise ValueError(f"kv4: the pool holds whole pages of {page} bytes")
-        if status is not None and (str(status.dtype) != "torch.int32" or status.numel() != 1 or
+        if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or
                                    status.device != pool.device):
             raise ValueError("kv4: status is one int32 on the pool's device")
         self.pool, self.status, self.device = pool, status, pool.device
         self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
-        self.pages = pool.numel() // page
+        self.pages, self._index = pool.numel() // page, pool.get_device()
         self.desc = Kv4CacheDesc(pool.device.index, q_heads, kv_heads, head_dim, self.pages, pool.data_ptr(),
                                  None if status is None else status.data_ptr())
         self._ref = C.byref(self.desc)
@@ -607,36 +624,39 @@ class Kv4Cache:
 
     def _stream(self, stream):
         if stream is None:
-            import torch
-            return torch.cuda.current_stream(self.device).cuda_stream
+            return self._current_stream(self._index).cuda_stream
         return getattr(stream, "cuda_stream", stream)
+
+    # The checks below run on every call: a decode step's kernels take less time than
+    # a few microseconds of them. Arguments are packed in the C struct's layout
+    # (ctypes sets fields one by one, three times as slow); a null pointer is 0.
 
     def _rows(self, x, name, tokens, heads, dtype=None):
         if x is None:
-            return Kv4Rows()
-        if x.device != self.device or x.dim() != 3 or tuple(x.shape) != (tokens, heads, self.head_dim):
+            return 0, 0, 0
+        if x.shape != (tokens, heads, self.head_dim) or x.get_device() != self._index:
             raise ValueError(f"kv4: {name} must be [{tokens}, {heads}, {self.head_dim}] on {self.device}")
         if dtype is not None and x.dtype != dtype:
             raise ValueError(f"kv4: {name} must be {dtype}")
         s = x.stride()
         if s[2] != 1 and x.numel():
             raise ValueError(f"kv4: the last dimension of {name} must be contiguous")
-        return Kv4Rows(x.data_ptr(), s[0], s[1])
+        return x.data_ptr(), s[0], s[1]
 
     def _array(self, x, name, dtype, shape=None, optional=False):
         """Pointer of a contiguous array."""
         if x is None:
             if optional:
-                return None
+                return 0
             raise ValueError(f"kv4: {name} is missing")
-        if x.device != self.device or str(x.dtype) != dtype or not x.is_contiguous():
+        if x.dtype != dtype or x.get_device() != self._index or not x.is_contiguous():
             raise ValueError(f"kv4: {name} must be a contiguous {dtype} tensor on {self.device}")
-        if shape is not None and tuple(x.shape) != shape:
+        if shape is not None and x.shape != shape:
             raise ValueError(f"kv4: {name} must be of shape {list(shape)}")
         return x.data_ptr()
 
     def _type(self, x, name):
-        code = _KV4_TYPES.get(str(x.dtype))
+        code = self._types.get(x.dtype)
         if code is None:
             raise ValueError(f"kv4: {name} must be float32, float16 or bfloat16")
         return code
@@ -652,59 +672,56 @@ class Kv4Cache:
         x = q if q is not None else k
         if x is None or (k is None) != (v is None) or (q is None) != (q_out is None):
             raise ValueError("kv4: append takes q with q_out, k with v, or all four")
-        T = x.shape[0]
-        one = "torch.float32"
-        args = Kv4AppendArgs(
-            self._rows(q, "q", T, self.q_heads, x.dtype), self._rows(k, "k", T, self.kv_heads, x.dtype),
-            self._rows(v, "v", T, self.kv_heads, x.dtype), self._type(x, "q"),
+        T, D, one, dtype = x.shape[0], self.head_dim, self._f32, x.dtype
+        args = _pack(
+            Kv4AppendArgs, _KV4_APPEND, *self._rows(q, "q", T, self.q_heads, dtype), *self._rows(k, "k", T, self.kv_heads, dtype),
+            *self._rows(v, "v", T, self.kv_heads, dtype), self._type(x, "q"),
             0 if q_out is None else self._type(q_out, "q_out"), T,
-            self._array(q_norm, "q_norm", one, (self.head_dim,), True),
-            self._array(k_norm, "k_norm", one, (self.head_dim,), True),
-            self._array(positions, "positions", "torch.int32", (T,), rope_dims == 0),
-            self._array(slots, "slots", "torch.int64", (T,), k is None),
-            None if q_out is None else self._array(q_out, "q_out", str(q_out.dtype), (T, self.q_heads, self.head_dim)),
+            self._array(q_norm, "q_norm", one, (D,), True), self._array(k_norm, "k_norm", one, (D,), True),
+            self._array(positions, "positions", self._i32, (T,), rope_dims == 0),
+            self._array(slots, "slots", self._i64, (T,), k is None),
+            0 if q_out is None else self._array(q_out, "q_out", q_out.dtype, (T, self.q_heads, D)),
             epsilon, theta, rope_dims, 0)
         _call("rs_qwen_kv4_append", self._ref, C.byref(args), self._stream(stream))
 
     def read(self, slots, k, v, stream=None):
         """Cached tokens back as values (rs_qwen_kv4_read): k, v [len(slots), kv_heads, D]."""
         shape = (slots.shape[0], self.kv_heads, self.head_dim)
-        _call("rs_qwen_kv4_read", self._ref, shape[0], self._array(slots, "slots", "torch.int64", shape[:1]),
-              self._type(k, "k"), self._array(k, "k", str(k.dtype), shape), self._array(v, "v", str(k.dtype), shape),
+        _call("rs_qwen_kv4_read", self._ref, shape[0], self._array(slots, "slots", self._i64, shape[:1]),
+              self._type(k, "k"), self._array(k, "k", k.dtype, shape), self._array(v, "v", k.dtype, shape),
               self._stream(stream))
 
     def attention(self, q, cu_seqlens, kv_lens, block_table, out, workspace, max_count: int, gate=None, lse=None,
                   weights_in=None, weights_out=None, scale: float = 0.0, stream=None):
         """Ragged causal attention over the pages (rs_qwen_kv4_attention). block_table: int32 [n_seq, pages];
         weights_in / weights_out: float32 [n_seq, kv_heads, columns]; workspace: uint8, workspace_bytes()."""
-        T, n, dim = q.shape[0], kv_lens.shape[0], q.dim()
-        if dim != 3 or block_table.dim() != 2:
+        if q.dim() != 3 or block_table.dim() != 2:
             raise ValueError("kv4: q must be [T, q_heads, head_dim] and block_table [n_seq, pages]")
-        if gate is not None and str(gate.dtype) != "torch.float32":
+        if gate is not None and gate.dtype != self._f32:
             raise ValueError("kv4: the gate must be float32")
-        one, whole = "torch.float32", "torch.int32"
+        T, n, pages, one, whole = q.shape[0], kv_lens.shape[0], block_table.shape[1], self._f32, self._i32
         columns = 0
         if weights_out is not None:
             columns = weights_out.shape[-1]
         elif weights_in is not None:
             raise ValueError("kv4: weights_in needs weights_out")
         wshape = (n, self.kv_heads, columns)
-        args = Kv4AttentionArgs(
-            self._rows(q, "q", T, self.q_heads), self._rows(gate, "gate", T, self.q_heads),
-            self._rows(out, "out", T, self.q_heads, q.dtype), self._type(q, "q"), 0, n, T, max_count,
+        args = _pack(
+            Kv4AttentionArgs, _KV4_ATTENTION, *self._rows(q, "q", T, self.q_heads), *self._rows(gate, "gate", T, self.q_heads),
+            *self._rows(out, "out", T, self.q_heads, q.dtype), self._type(q, "q"), 0, n, T, max_count,
             self._array(cu_seqlens, "cu_seqlens", whole, (n + 1,)), self._array(kv_lens, "kv_lens", whole, (n,)),
-            self._array(block_table, "block_table", whole, (n, block_table.shape[1])), block_table.shape[1], scale,
+            self._array(block_table, "block_table", whole, (n, pages)), pages, scale,
             self._array(lse, "lse", one, (T, self.q_heads), True),
             self._array(weights_in, "weights_in", one, wshape, True),
             self._array(weights_out, "weights_out", one, wshape, True), columns,
-            self._array(workspace, "workspace", "torch.uint8"), workspace.numel())
+            self._array(workspace, "workspace", self._u8), workspace.numel())
         _call("rs_qwen_kv4_attention", self._ref, C.byref(args), self._stream(stream))
 
     def evict(self, kv_lens, src_table, dst_table, weights, keep: int, recent: int, kept, new_lens, weights_out=None,
               stream=None):
         """Keeps the most attended keys of every sequence and KV head (rs_qwen_kv4_evict); the kept keys move to
         the pages of dst_table."""
-        n, one, whole = kv_lens.shape[0], "torch.float32", "torch.int32"
+        n, one, whole = kv_lens.shape[0], self._f32, self._i32
         args = Kv4EvictArgs(
             n, self._array(kv_lens, "kv_lens", whole, (n,)),
             self._array(src_table, "src_table", whole, (n, src_table.shape[1])), src_table.shape[1],

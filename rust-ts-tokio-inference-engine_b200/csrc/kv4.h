@@ -113,6 +113,7 @@ struct Kv4AttentionArgs {
   void* workspace = nullptr;
   size_t workspace_bytes = 0;
   int sm_count = 0;
+  bool coarse = false;  // fp16 queries may run in kv4_chunk.cu: their output feeds something coarser than fp16
   int row_limit = INT_MAX;  // sequences with more query rows per KV head run in kv4_chunk.cu
 };
 // Sequences above row_limit, tcgen05 tiles of 128 rows (no lse, no weights).

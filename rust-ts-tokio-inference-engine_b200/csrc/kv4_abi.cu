@@ -180,7 +180,7 @@ int rs_qwen_kv4_attention(const rs_qwen_kv4_cache* cache, const rs_qwen_kv4_atte
          "kv4 attention: too many sequences or tokens");
     if (!args->n_seq || !args->tokens) return;
     need(args->q.data && args->out.data, "kv4 attention: queries or output missing");
-    need(args->max_count >= 1 && args->max_count <= args->tokens, "kv4 attention: max_count must be 1 to tokens");
+    need(args->max_count >= 1, "kv4 attention: max_count must be positive");
     need(args->cu_seqlens && args->kv_lens && args->block_table && aligned(args->cu_seqlens, 4) &&
              aligned(args->kv_lens, 4) && aligned(args->block_table, 4),
          "kv4 attention: cu_seqlens, kv_lens or block_table missing or not 4-byte aligned");
@@ -206,7 +206,7 @@ int rs_qwen_kv4_attention(const rs_qwen_kv4_cache* cache, const rs_qwen_kv4_atte
     a.type = args->dtype;
     a.n_seq = int(args->n_seq);
     a.tokens = int(args->tokens);
-    a.max_count = int(args->max_count);
+    a.max_count = int(std::min(args->max_count, args->tokens));
     a.cu_seqlens = args->cu_seqlens;
     a.kv_lens = args->kv_lens;
     a.table = args->block_table;

@@ -24,12 +24,17 @@
 //   masked the same way. The step of V is folded into the weights, P_g = p
 //   scale_g, rounded to fp16 (2^-11 of a weight, the operand's own precision)
 //   after a power of two per group has brought the scales that the warp has seen
-//   to at most 2^6; sum p bias_g is kept in 32 bits beside it.
+//   to at most 2^6; sum p bias_g is kept in 32 bits beside it. Since n is not
+//   centred, that rounding moves a row by 2^-11 of twice its size, which bf16
+//   rows do not show but fp16 rows do (4.6e-4 relative to 64 bits for 33
+//   sequences of head_dim 128, of which fp16's own rounding is 2.1e-4): for fp16
+//   what the rounding left out is multiplied too.
 // The running maximum moves only when a logit exceeds it by 2^8: a vote per
 // page then replaces the reduction over the keys, and the weights stay below
 // 2^8 x 2^6, inside fp16.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "kv4_device.cuh"
 
@@ -109,6 +114,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
   pdl_trigger();
   pdl_wait();
   using L = Kv4Layout<D>;
+  constexpr bool kFine = std::is_same_v<T, __half>;
   constexpr int NG = L::kGroups, LW = L::kLaneWords;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   Smem<D>& sm = *reinterpret_cast<Smem<D>*>(smem_raw);
@@ -501,13 +507,19 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t pb[NG][2];
+        uint32_t pb[NG][2], rest[kFine ? NG : 1][2];
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const float step = kv4_scale(vm[2 * h + k][g]) * vinv[g];
-            pb[g][k] = transpose8x8(pack_f16(s[2 * h + k][0] * step, s[2 * h + k][1] * step));
+            const float p0 = s[2 * h + k][0] * step, p1 = s[2 * h + k][1] * step;
+            const uint32_t p = pack_f16(p0, p1);
+            pb[g][k] = transpose8x8(p);
+            if (kFine) {
+              const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&p));
+              rest[g][k] = transpose8x8(pack_f16(p0 - r.x, p1 - r.y));
+            }
           }
         // nibbles of keys 2 tq, 2 tq + 1 (even places first) and 2 tq + 8, 2 tq + 9
         alignas(16) uint32_t w[4][NG];
@@ -521,9 +533,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
             uint32_t x = __byte_perm(w[0][g], w[1][g], b ? 0x7632 : 0x5410);
             uint32_t y = __byte_perm(w[2][g], w[3][g], b ? 0x7632 : 0x5410);
             mma_f16(o[g][2 * b], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, pb[g][0], pb[g][1]);
+            if (kFine) mma_f16(o[g][2 * b], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, rest[g][0], rest[g][1]);
             x >>= 8;
             y >>= 8;
             mma_f16(o[g][2 * b + 1], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, pb[g][0], pb[g][1]);
+            if (kFine) mma_f16(o[g][2 * b + 1], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, rest[g][0], rest[g][1]);
           }
       }
       __syncwarp();
@@ -900,7 +914,10 @@ size_t decode_workspace(int Hq, int Hkv, int D, size_t n_seq, size_t tokens, int
 // asked for: five tiles, for each of which this kernel reads the pages again. From
 // six on the 128-row tiles of kv4_chunk_kernel are faster: 64 sequences of 4096
 // keys at head_dim 256 take 137 us here with 32 rows and 169 there, 194 and 171
-// with 48.
+// with 48. Only bf16 rows go there: its fp16 operands (keys, values, weights)
+// leave 3.5e-4 of error, nothing beside bf16's own rounding (1.7e-3) and twice
+// fp16's (2.1e-4). That precision has its price: 2048 fp16 tokens behind 16384
+// keys take 6.2 ms here, bf16 ones 0.79 ms there (256 behind 4096: 262 and 77 us).
 constexpr int kChunkRows = 40;
 
 template <int D, class T>
@@ -911,7 +928,7 @@ void attend(const Kv4AttentionArgs& a, cudaStream_t s) {
   });
   Kv4AttentionArgs b = a;
   const int G = a.cache.Hq / a.cache.Hkv, ctas = a.sm_count * kCtasPerSm;
-  const bool chunks = !a.lse && !a.weights_out && a.max_count * int64_t(G) > kChunkRows;
+  const bool chunks = (a.type == kKv4BF16 || a.coarse) && !a.lse && !a.weights_out && a.max_count * int64_t(G) > kChunkRows;
   b.row_limit = chunks ? kChunkRows : INT_MAX;
   const int tiles = (int(std::min(int64_t(a.max_count) * G, int64_t(b.row_limit))) + kRowsPerTile - 1) / kRowsPerTile;
   if (int64_t(a.n_seq) * a.cache.Hkv * tiles > (int64_t(1) << 30) / (a.table_stride / 2 + 1 + kUnitPairs))

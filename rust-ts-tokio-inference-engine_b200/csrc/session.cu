@@ -640,6 +640,7 @@ struct Session {
     t.table = kv4_table.p;
     t.table_stride = bt_stride;
     t.scale = 1.f / std::sqrt(float(d.D));
+    t.coarse = true;  // as the other fp16 operands of the projections
     if (kv4_track) {
       t.weights_in = t.weights_out = kv4_layer_weights(ly.type_index);
       t.weights_stride = d.ctx;

@@ -608,7 +608,7 @@ def test_wrapper_refusals(pkg):
 
     call()
     for kw in (dict(q=q.float()), dict(out=torch.empty_like(q).float()), dict(kv_lens=seqs.kv_lens.long()),
-               dict(block_table=seqs.table[:, ::2]), dict(cu_seqlens=cu[:1]), dict(gate=q), dict(max_count=2),
+               dict(block_table=seqs.table[:, ::2]), dict(cu_seqlens=cu[:1]), dict(gate=q), dict(max_count=0),
                dict(workspace=ws[:8]), dict(q=q[:, :2]), dict(q=q.cpu()), dict(lse=torch.empty(1, 3, device="cuda")),
                dict(weights_in=torch.empty(1, 1, 16, device="cuda")), dict(q=q.transpose(1, 2).contiguous().transpose(1, 2))):
         with pytest.raises((ValueError, pkg.NativeError)):

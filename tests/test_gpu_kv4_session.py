@@ -145,6 +145,36 @@ def test_steps_against_the_oracle(pkg, O, make, block, track):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("track", [False, True])
+def test_wide_heads_against_the_oracle(pkg, O, track):
+    """16 query heads and 2 KV heads of 256: a prefill, a block of 40 tokens (128-row tiles without tracking) and
+    single tokens."""
+    if not has_cuda():
+        pytest.skip("no CUDA device")
+    O.set_routing_slack(5e-2)
+    cfg = pkg.config1(layers=4, context=256)
+    store = pkg.WeightStore().synthetic(cfg, SEED)
+    s = pkg.DeviceSession(store, cfg, slots=4, budget_bytes=1 << 28).kv4(track)
+    model = O.Model(O.config1(layers=4, context=256), SEED)
+    try:
+        s.set_capture(True)
+        toks = np.random.default_rng(3).integers(0, cfg.vocab, size=72).astype(np.uint32)
+        cur, state, pos = None, None, 0
+        for n in (30, 40, 1, 1):
+            (cur,), _, logits = s.step_ragged([cur], [pos], [n], toks[pos:pos + n],
+                                              flags=pkg.RAGGED_LOGITS | pkg.RAGGED_ALL_ROWS)
+            route = s.debug_routing(n)
+            held = np.stack(s.kv4_read(cur, 0)[:2])[None, :, :, pos:]
+            lg, _, _, _ = model.forward(toks[pos:pos + n], pos, old_state=state, forced_routing=route, cached_kv=held)
+            assert max(rel_l2(logits[j], lg[j]) for j in range(n)) <= 1e-2
+            state, pos = s.snapshot(cur), pos + n
+        s.release(cur)
+    finally:
+        s.close()
+        store.close()
+
+
+@pytest.mark.gpu
 def test_forks_copy_the_shared_page(pkg, make):
     s = make()
     toks = prompt(21)

@@ -566,9 +566,10 @@ class DeviceSession:
 # ---- 4-bit paged KV cache ----
 
 KV4_PAGE = 16  # tokens per page
-# Kv4AppendArgs and Kv4AttentionArgs in one call
+# the argument structs, packed in one call
 _KV4_APPEND = struct.Struct("=" + 3 * "Qqq" + "IIQQQQQQffii")
 _KV4_ATTENTION = struct.Struct("=" + 3 * "Qqq" + "IIQQQQQQqf4xQQQqQQ")
+_KV4_EVICT = struct.Struct("=QQQqQqQqiiQQQq")
 
 
 def _pack(kind, layout, *values):
@@ -579,6 +580,7 @@ def _pack(kind, layout, *values):
 
 
 assert _KV4_APPEND.size == C.sizeof(Kv4AppendArgs) and _KV4_ATTENTION.size == C.sizeof(Kv4AttentionArgs)
+assert _KV4_EVICT.size == C.sizeof(Kv4EvictArgs)
 
 
 def kv4_page_bytes(kv_heads: int, head_dim: int) -> int:
@@ -722,8 +724,8 @@ class Kv4Cache:
         """Keeps the most attended keys of every sequence and KV head (rs_qwen_kv4_evict); the kept keys move to
         the pages of dst_table."""
         n, one, whole = kv_lens.shape[0], self._f32, self._i32
-        args = Kv4EvictArgs(
-            n, self._array(kv_lens, "kv_lens", whole, (n,)),
+        args = _pack(
+            Kv4EvictArgs, _KV4_EVICT, n, self._array(kv_lens, "kv_lens", whole, (n,)),
             self._array(src_table, "src_table", whole, (n, src_table.shape[1])), src_table.shape[1],
             self._array(dst_table, "dst_table", whole, (n, dst_table.shape[1])), dst_table.shape[1],
             self._array(weights, "weights", one, (n, self.kv_heads, weights.shape[-1])), weights.shape[-1], keep, recent,

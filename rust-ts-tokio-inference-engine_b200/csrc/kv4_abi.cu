@@ -176,7 +176,8 @@ int rs_qwen_kv4_attention(const rs_qwen_kv4_cache* cache, const rs_qwen_kv4_atte
     a.cache = view(cache);
     need(args, "kv4 attention: null arguments");
     need(args->dtype == RS_QWEN_F16 || args->dtype == RS_QWEN_BF16, "kv4 attention: queries must be fp16 or bf16");
-    need(args->n_seq <= size_t(INT32_MAX) / size_t(cache->kv_heads) && args->tokens <= size_t(INT32_MAX),
+    need(args->n_seq <= size_t(INT32_MAX) / size_t(cache->kv_heads) &&
+             args->tokens <= size_t(INT32_MAX) / size_t(cache->q_heads),
          "kv4 attention: too many sequences or tokens");
     if (!args->n_seq || !args->tokens) return;
     need(args->q.data && args->out.data, "kv4 attention: queries or output missing");

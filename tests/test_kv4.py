@@ -90,7 +90,8 @@ def attention(pkg, **kw):
 
 
 @pytest.mark.parametrize("kw,match", [
-    (dict(dtype=0), "fp16 or bf16"), (dict(dtype=9), "fp16 or bf16"), (dict(max_count=0), "max_count"),
+    (dict(dtype=0), "fp16 or bf16"), (dict(dtype=9), "fp16 or bf16"), (dict(tokens=1 << 29), "tokens"), (dict(n_seq=1 << 30), "sequences"),
+    (dict(max_count=0), "max_count"),
     (dict(cu_seqlens=None), "cu_seqlens"), (dict(kv_lens=FAKE + 2), "kv_lens"),
     (dict(block_table=None), "block_table"), (dict(table_stride=0), "table_stride"),
     (dict(table_stride=1 << 28), "table_stride"), (dict(scale=-1.0), "scale"), (dict(scale=float("inf")), "scale"),

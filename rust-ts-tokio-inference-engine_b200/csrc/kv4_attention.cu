@@ -917,7 +917,7 @@ size_t decode_workspace(int Hq, int Hkv, int D, size_t n_seq, size_t tokens, int
 // with 48. Only bf16 rows go there: its fp16 operands (keys, values, weights)
 // leave 3.5e-4 of error, nothing beside bf16's own rounding (1.7e-3) and twice
 // fp16's (2.1e-4). That precision has its price: 2048 fp16 tokens behind 16384
-// keys take 6.2 ms here, bf16 ones 0.79 ms there (256 behind 4096: 262 and 77 us).
+// keys take 6.2 ms here, bf16 ones 0.71 ms there (256 behind 4096: 262 and 73 us).
 constexpr int kChunkRows = 40;
 
 template <int D, class T>

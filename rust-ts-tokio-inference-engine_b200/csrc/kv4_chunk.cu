@@ -8,9 +8,13 @@
 //   S[128 x 64] = Q K^T   Q in TMEM (128 columns), K in shared memory
 //   O[128 x D] += P V     P in TMEM, V^T in shared memory, O in TMEM (D columns)
 // so each MMA reads only its B operand from shared memory. Warp roles:
-//   0-3   softmax: one thread per row; running maximum and sum in registers
-//   4-7   dequantisation of K, 8-11 of V: nibbles -> fp16 operands in the 128B-swizzled layout
-//   12    MMA issue    13, 14  bulk copies of the pages' K and V parts
+//   0-7   softmax: two threads per row, each with half of a block's keys; they tell
+//         each other their maximum, so both hold the row's; sums in registers
+//   8-11  dequantisation of K, 12-15 of V: nibbles -> fp16 operands in the 128B-swizzled layout
+//   16    MMA issue    17, 18  bulk copies of the pages' K and V parts
+// 2048 tokens of 16 + 2 heads of 256 behind 14336 keys: 710 us (0.73 PFLOP/s; 778
+// with one softmax thread per row). What is left is the chain of a block in the
+// dequantisation warps: steps, meeting, values.
 // The nibbles of the page layout come out as the operands' element pairs: two
 // dims of a K row, two keys of a V^T row. Masked, a pair is an fp16 subnormal
 // pair n 2^-24 (or n 2^-20), so one fused multiply-add with the step times 2^24
@@ -34,9 +38,9 @@ extern std::atomic<uint64_t> g_kernel_launches;
 namespace {
 
 constexpr int kRows = 128, kKeys = 64, kBlockPages = kKeys / kPageTokens;
-constexpr int kSoftWarps = 4, kDeqWarps = 4, kMmaWarp = 12, kLoadK = 13, kLoadV = 14;
-constexpr int kThreads = 16 * 32;  // the last warp only completes its warpgroup
-constexpr int kSoftRegs = 152, kOtherRegs = 120;  // of 512 x 128 registers at launch: 128 x (152 + 3 x 120)
+constexpr int kSoftWarps = 8, kDeqWarps = 4, kMmaWarp = 16, kLoadK = 17, kLoadV = 18;
+constexpr int kThreads = 20 * 32;  // the last warp only completes its warpgroup
+constexpr int kSoftRegs = 104, kOtherRegs = 88;  // of 640 x 96 registers at launch: 256 x 104 + 384 x 88
 constexpr int kRaw = 3;         // raw page stages, K and V each
 constexpr int kSets = 2;        // sets of steps and biases, K and V each
 constexpr int kUnitBlocks = 4;  // what a unit costs beside its blocks, in blocks
@@ -105,7 +109,8 @@ struct Smem {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full, s_empty, p_full[2], p_empty[2], q_full, o_empty;
   uint32_t tmem;
   int abort;
-  int scan[16];
+  int scan[kThreads / 32];
+  float top[2][2][kRows], sum[2][kRows];    // what the two threads of a row tell each other
   int offsets[kGroupsMax + 1];
 };
 
@@ -269,6 +274,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
   pdl_trigger();  // not before the TMEM is taken: a dependent kernel's CTA could hold it and wait for this one
   const uint32_t tmem = sm.tmem;
   volatile int* abort = &sm.abort;
+  // False when the wait ran out, here or in another warp (the status word has it).
+  // Warps that meet others at a barrier go on all the same, on whatever the shared
+  // memory holds and with no further waiting, so that none is left there.
   auto wait = [&](uint64_t* bar, uint32_t parity) { return kv4_wait(bar, parity, a.cache.status, abort); };
 
   if (warp < kSoftWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
@@ -405,7 +413,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
     // Steps and biases of block n as fp16 operands, one set ahead of its values: a
     // warp per group, a lane for keys lane and lane + 32.
     auto scales = [&](const Seq& q, int j, bool first) {
-      if (!wait(&sm.kraw_full[n % kRaw], n / kRaw & 1)) return false;
+      wait(&sm.kraw_full[n % kRaw], n / kRaw & 1);
+      __syncwarp();
       if (dw < NG) {
         float most = 0.f;
         uint32_t own[2];
@@ -431,11 +440,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
         if (dt == 0) sm.kinfo[n & 7] = make_float2(power.e == kNone ? 0.f : pow2i(power.e - 16), __int_as_float(sm.absent[n & 7]));
       }
       asm volatile("bar.sync 1, %0;" ::"n"(kDeqWarps * 32) : "memory");
-      return true;
     };
     auto values = [&] {
       const int st = n % kRaw;
-      if (n >= 2 && !wait(&sm.k_empty[n & 1], (n / 2 - 1) & 1)) return false;
+      if (n >= 2) wait(&sm.k_empty[n & 1], (n / 2 - 1) & 1);
+      __syncwarp();
       const int t = dt % 4;
       alignas(16) uint32_t w[2][LW];
 #pragma unroll
@@ -471,12 +480,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
         mbar_arrive(&sm.k_full[n & 1]);
       }
       ++n;
-      return true;
     };
     for_units([&](const Cursor&, const Seq& q, int j0, int blocks, bool, int) {
-      if (blocks && !scales(q, j0, true)) return false;
-      for (int j = 0; j < blocks; ++j)
-        if (!values() || (j + 1 < blocks && !scales(q, j0 + j + 1, false))) return false;
+      if (blocks) scales(q, j0, true);
+      for (int j = 0; j < blocks; ++j) {
+        values();
+        if (j + 1 < blocks) scales(q, j0 + j + 1, false);
+      }
       return true;
     });
   } else if (warp >= kSoftWarps + kDeqWarps && warp < kMmaWarp) {
@@ -484,7 +494,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
     uint32_t n = 0;
     Power power;  // of this warp's group
     auto scales = [&](const Seq& q, int j, bool first) {  // a warp per group, a lane per pair of keys
-      if (!wait(&sm.vraw_full[n % kRaw], n / kRaw & 1)) return false;
+      wait(&sm.vraw_full[n % kRaw], n / kRaw & 1);
+      __syncwarp();
       if (dw < NG) {
         const int tok = lane * 2 % kPageTokens, page = lane * 2 / kPageTokens;
         const uint8_t* raw = sm.vraw[n % kRaw][page] + Smem<D>::kHalf + tok * NG * 4 + dw * 4;
@@ -513,11 +524,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
         sm.vflags[n & 7][dw] = 0;
       }
       asm volatile("bar.sync 2, %0;" ::"n"(kDeqWarps * 32) : "memory");
-      return true;
     };
     auto values = [&] {
       const int st = n % kRaw;
-      if (n >= 2 && !wait(&sm.v_empty[n & 1], (n / 2 - 1) & 1)) return false;
+      if (n >= 2) wait(&sm.v_empty[n & 1], (n / 2 - 1) & 1);
+      __syncwarp();
 #pragma unroll 1
       for (int part = dw; part < 2 * NG; part += kDeqWarps) {
         // Lane = (word of four, octet of keys). A lane takes its octet's four key
@@ -553,18 +564,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
         mbar_arrive(&sm.v_full[n & 1]);
       }
       ++n;
-      return true;
     };
     for_units([&](const Cursor&, const Seq& q, int j0, int blocks, bool, int) {
-      if (blocks && !scales(q, j0, true)) return false;
-      for (int j = 0; j < blocks; ++j)
-        if (!values() || (j + 1 < blocks && !scales(q, j0 + j + 1, false))) return false;
+      if (blocks) scales(q, j0, true);
+      for (int j = 0; j < blocks; ++j) {
+        values();
+        if (j + 1 < blocks) scales(q, j0 + j + 1, false);
+      }
       return true;
     });
   } else if (warp < kSoftWarps) {
-    const int row = warp * 32 + lane;
-    const uint32_t lanes = tmem + (uint32_t(warp * 32) << 16);
+    // two threads per row, each with half of a block's keys and of O's dims
+    const int quadrant = warp & 3, half = warp >> 2, row = quadrant * 32 + lane;
+    const uint32_t lanes = tmem + (uint32_t(quadrant * 32) << 16);
     uint32_t n = 0;
+    auto both = [&] { asm volatile("bar.sync %0, 64;" ::"r"(3 + quadrant) : "memory"); };
+    constexpr int kMine = kKeys / 2;
     for_units([&](const Cursor& u, const Seq& q, int j0, int blocks, bool whole, int slot) {
       const int at = u.r * kRows + row, token = at / G, head = u.g * G + at % G;
       const bool real = token < q.count;
@@ -595,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
         const int e = most && fine ? int(most >> 23) - 126 : 0;
         const float up = pow2i((14 - e) / 2), up2 = fine ? pow2i(14 - e - (14 - e) / 2) : 0.f;
 #pragma unroll 1
-        for (int d = 0; d < D; d += 64) {
+        for (int d = 64 * half; d < D; d += 128) {
           uint32_t v[32];
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
@@ -617,16 +632,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
         const int least = __reduce_min_sync(0xffffffffu, seen);
         uint32_t poison = 0u;  // groups of which the row sees a NaN
         for (int j = j0; j < j0 + blocks; ++j, ++n) {
-          if (!wait(&sm.s_full, n & 1)) return false;
+          wait(&sm.s_full, n & 1);
           tc_fence_after();
-          float2 x[kKeys / 2];
+          float2 x[kMine / 2];
           {
-            uint32_t s[kKeys];
-            tmem_ld32(lanes + kTmS, s);
-            tmem_ld32(lanes + kTmS + 32, s + 32);
+            uint32_t s[kMine];
+            __syncwarp();
+            tmem_ld32(lanes + kTmS + kMine * half, s);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < kKeys / 2; ++i) x[i] = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+            for (int i = 0; i < kMine / 2; ++i) x[i] = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
           }
           tc_fence_before();
           const float2 info = sm.kinfo[n & 7];
@@ -634,20 +649,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
           float fk = fine ? fmaxf(f1 * info.x, FLT_MIN) : NAN;  // above zero: a masked -infinity stays one
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.s_empty);
-          const int key0 = j * kKeys;
-          if (key0 + kKeys > least || absent) {
+          const int key0 = j * kKeys + kMine * half;
+          if (key0 + kMine > least || absent) {
+            const int gone = absent >> (kMine / kPageTokens * half);
 #pragma unroll
-            for (int i = 0; i < kKeys / 2; ++i) {
-              if (key0 + 2 * i >= seen || (absent >> (2 * i / kPageTokens) & 1)) x[i].x = -INFINITY;
-              if (key0 + 2 * i + 1 >= seen || (absent >> (2 * i / kPageTokens) & 1)) x[i].y = -INFINITY;
+            for (int i = 0; i < kMine / 2; ++i) {
+              if (key0 + 2 * i >= seen || (gone >> (2 * i / kPageTokens) & 1)) x[i].x = -INFINITY;
+              if (key0 + 2 * i + 1 >= seen || (gone >> (2 * i / kPageTokens) & 1)) x[i].y = -INFINITY;
             }
           }
           float tops[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) tops[i] = fmaxf(x[i].x, x[i].y);
 #pragma unroll
-          for (int i = 4; i < kKeys / 2; ++i) tops[i % 4] = fmaxf(fmaxf(tops[i % 4], x[i].x), x[i].y);
-          const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * fk;
+          for (int i = 4; i < kMine / 2; ++i) tops[i % 4] = fmaxf(fmaxf(tops[i % 4], x[i].x), x[i].y);
+          float most = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+          sm.top[n & 1][half][row] = most;
+          both();
+          most = fmaxf(most, sm.top[n & 1][half ^ 1][row]);
+          const float top = most * fk;
           const bool grow = top > m + kLazy;
           float shrink = 1.f;
           if (grow) {
@@ -659,14 +679,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
           // for the whole row. Beyond 2^24 that could be large: round the products first.
           if (__any_sync(0xffffffffu, fabsf(m) > 16777216.f && m > -FLT_MAX)) {
 #pragma unroll
-            for (int i = 0; i < kKeys / 2; ++i) x[i] = make_float2(x[i].x * fk, x[i].y * fk);
+            for (int i = 0; i < kMine / 2; ++i) x[i] = make_float2(x[i].x * fk, x[i].y * fk);
             fk = 1.f;
           }
           // weights, packed octet by octet in V^T's order of the key pairs
           float2 sum = make_float2(0.f, 0.f);
-          uint32_t p[kKeys / 2];
+          uint32_t p[kMine / 2];
 #pragma unroll
-          for (int o = 0; o < kKeys / 8; ++o) {
+          for (int o = 0; o < kMine / 8; ++o) {
 #pragma unroll
             for (int i = 4 * o; i < 4 * o + 4; ++i) {
               x[i] = fma2(x[i], make_float2(fk, fk), make_float2(-m, -m));
@@ -682,8 +702,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
           }
           l += sum.x + sum.y;
           // With V of this block in place the MMAs on the block before the last are done, so P's buffer is free too
-          if (!wait(&sm.v_full[n & 1], n / 2 & 1)) return false;
-          tmem_st32(lanes + kTmP + (n & 1) * 32, p);
+          wait(&sm.v_full[n & 1], n / 2 & 1);
+          __syncwarp();
+          tmem_st16(lanes + kTmP + (n & 1) * 32 + kMine / 2 * half, p);
           const uint32_t flags = *reinterpret_cast<const uint32_t*>(sm.vflags[n & 7]);
           const bool moved = flags & 0x01010101u;
           if (flags & 0x02020202u) {
@@ -691,14 +712,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
             for (int g = 0; g < NG; ++g)
 #pragma unroll 1
               for (int i = 0; i < kKeys; ++i)
-                if ((sm.vnan[n & 7][g][i & 1] >> (i / 2) & 1) && key0 + i < seen) poison |= 1u << g;
+                if ((sm.vnan[n & 7][g][i & 1] >> (i / 2) & 1) && j * kKeys + i < seen) poison |= 1u << g;
           }
           if (j > j0 && (moved || __any_sync(0xffffffffu, grow))) {
             // O so far to the new maximum and powers, when the MMAs on it are done
-            if (!wait(&sm.p_empty[(n - 1) & 1], ((n - 1) / 2) & 1)) return false;
+            wait(&sm.p_empty[(n - 1) & 1], ((n - 1) / 2) & 1);
+            __syncwarp();
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
+            for (int c = D / 2 * half; c < D / 2 * (half + 1); c += 32) {
               const int was = sm.ve_was[n & 7][c / 64];
               const float f = shrink * (was == kNone ? 1.f : pow2i(was - sm.ve[n & 7][c / 64]));
               uint32_t v[32];
@@ -715,12 +737,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
           if (lane == 0) mbar_arrive(&sm.p_full[n & 1]);
         }
         // the rows
-        if (!wait(&sm.p_empty[(n - 1) & 1], ((n - 1) / 2) & 1)) return false;
+        wait(&sm.p_empty[(n - 1) & 1], ((n - 1) / 2) & 1);
+        sm.sum[half][row] = l;
+        both();
+        l += sm.sum[half ^ 1][row];
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const size_t part = (size_t(blockIdx.x) * 2 + slot) * kRows + row;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
+        for (int c = D / 2 * half; c < D / 2 * (half + 1); c += 16) {
           uint32_t v[16];
           tmem_ld16(lanes + kTmO + c, v);
           tmem_wait_ld();
@@ -749,7 +774,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.o_empty);
       }
-      if (!whole && real) {
+      if (!whole && real && half == 0) {
         const size_t part = (size_t(blockIdx.x) * 2 + slot) * kRows + row;
         ws.ml[part] = make_float2(m, l);
         if (!blocks)

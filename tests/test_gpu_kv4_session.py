@@ -219,6 +219,29 @@ def test_verify_accept(pkg, make):
         assert np.array_equal(s.snapshot(made[i]), s.snapshot(chains[i][a]))
 
 
+@pytest.mark.gpu
+def test_draft_head_beside_4_bit_pages(pkg, O, make, store):
+    """The MTP head drafts from hidden rows of a 4-bit session, on bf16 pages of its own."""
+    O.set_routing_slack(5e-2)
+    s, model = make(), O.Model(tiny(O), SEED, mtp=True)
+    s.mtp_attach(store)
+    n = 6
+    (target,), _, _ = s.step_ragged([None], [0], [n], prompt(n), flags=pkg.RAGGED_SAMPLED | pkg.RAGGED_HIDDEN)
+    before = s.snapshot(target)
+    s.set_capture(True)
+    draft, logits = s.mtp_step(None, target, prompt(n, 6))
+    kv = np.zeros(2 * PER, np.float64)
+    want, hidden = model.mtp_forward(prompt(n, 6), 0, s.hidden_snapshot(target, n).astype(np.float64), kv,
+                                     forced_routing=s.debug_routing(n)[0])
+    assert rel_l2(logits, want[-1]) <= 1e-2
+    k, v, rows = s.mtp_snapshot(draft, n)
+    kv = kv.reshape(2, KV_HEADS, CONTEXT, DIM)
+    assert rel_l2(rows, hidden) <= 1e-2 and rel_l2(k[:, :n], kv[0, :, :n]) <= 1e-2 and rel_l2(v[:, :n], kv[1, :, :n]) <= 1e-2
+    assert np.array_equal(s.snapshot(target), before)
+    s.mtp_release(draft)
+    s.release(target)
+
+
 def rotated(k, by):
     """Keys [.., d] moved `by` positions along the rotation (64 bits)."""
     j = np.arange(ROPE // 2)

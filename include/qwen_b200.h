@@ -510,7 +510,7 @@ int rs_qwen_kv4_read(const rs_qwen_kv4_cache* cache, size_t tokens, const int64_
  * the call's query rows of its KV head; the newest n keys start from zero.
  * weights_in may be weights_out. Columns from kv_lens[s] on are not written.
  * Sums are fp32. For bf16 without lse and weights, sequences that feed more than
- * 40 query rows per KV head (max_count x q_heads / kv_heads) run on larger tiles,
+ * 32 query rows per KV head (max_count x q_heads / kv_heads) run on larger tiles,
  * which round keys, values and softmax weights to fp16 (2^-11 each). All others
  * use the stored nibbles exactly, with softmax weights to 2^-11 (bf16) or 2^-22
  * (fp16): ask for bf16 where long prefills should be fast. max_count may be

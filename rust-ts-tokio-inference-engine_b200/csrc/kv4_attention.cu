@@ -911,14 +911,15 @@ size_t decode_workspace(int Hq, int Hkv, int D, size_t n_seq, size_t tokens, int
 }
 
 // Rows of a sequence up to which it runs here when neither lse nor weights are
-// asked for: five tiles, for each of which this kernel reads the pages again. From
-// six on the 128-row tiles of kv4_chunk_kernel are faster: 64 sequences of 4096
-// keys at head_dim 256 take 137 us here with 32 rows and 169 there, 194 and 171
-// with 48. Only bf16 rows go there: its fp16 operands (keys, values, weights)
-// leave 3.5e-4 of error, nothing beside bf16's own rounding (1.7e-3) and twice
-// fp16's (2.1e-4). That precision has its price: 2048 fp16 tokens behind 16384
-// keys take 6.2 ms here, bf16 ones 0.71 ms there (256 behind 4096: 262 and 73 us).
-constexpr int kChunkRows = 40;
+// asked for: four tiles, for each of which this kernel reads the pages again. From
+// five on the 128-row tiles of kv4_chunk_kernel are faster: 64 sequences of 4096
+// keys take 129 us here with 32 rows and 134 there, 158 and 137 with 40 (2 KV heads
+// of 256), 155 and 184, 191 and 186 (4 of 128). Only bf16 rows go there: its fp16
+// operands (keys, values, weights) leave 3.5e-4 of error, nothing beside bf16's own
+// rounding (1.7e-3) and twice fp16's (2.1e-4). That precision has its price: 2048
+// fp16 tokens behind 14336 keys take 6.2 ms here, bf16 ones 0.71 ms there (256
+// behind 3840: 262 and 73 us).
+constexpr int kChunkRows = 32;
 
 template <int D, class T>
 void attend(const Kv4AttentionArgs& a, cudaStream_t s) {

@@ -118,7 +118,7 @@ def check_attention(seqs, q, cu, out, lse=None, weights=None, weights_in=None, g
     is a 32-bit sum (ds, from attention()); the softmax weights times a value's step are rounded to fp16 (half a
     step: 2^-11 of at most 15 steps of the value's group, i.e. of the range it spans); the exponential and the
     sigmoid have a relative error below 2^-18; the result is rounded once to its type. Without lse and weights a
-    sequence of more than 40 query rows per KV head goes through fp16 operands of K and V: each value is off by at
+    sequence of more than 32 query rows per KV head goes through fp16 operands of K and V: each value is off by at
     most half a step, 2^-11 of it, so a logit by 2^-11 of the sum of |q| |k| (ds is D 2^-23 of it: 2^12 / D times as
     much) and an output by 2^-11 of the largest value."""
     scale = scale or seqs.D ** -0.5
@@ -129,7 +129,7 @@ def check_attention(seqs, q, cu, out, lse=None, weights=None, weights_in=None, g
         k, v = seqs.k[s], seqs.v[s]
         ref, ref_lse, ref_w, ds = attention(q[a:z], k, v, seqs.most[s], scale)
         vmax = v.abs().amax().item() if n else 0.0
-        chunk = lse is None and weights is None and (z - a) * G > 40
+        chunk = lse is None and weights is None and (z - a) * G > 32 and out.dtype == torch.bfloat16
         if chunk:
             ds = ds * (1 + 2.0 ** 12 / seqs.D)
         loose = 2.0 ** -11 * (3 if chunk else 2) * vmax + (2 * ds[..., None] + 2.0 ** -18) * vmax

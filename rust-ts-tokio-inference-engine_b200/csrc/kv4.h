@@ -116,6 +116,11 @@ struct Kv4AttentionArgs {
   bool coarse = false;  // fp16 queries may run in kv4_chunk.cu: their output feeds something coarser than fp16
   int row_limit = INT_MAX;  // sequences with more query rows per KV head run in kv4_chunk.cu
 };
+// Throws std::invalid_argument for a call beyond the 32-bit places that its kernels
+// count in, before any of them is launched (host values only; launch_kv4_attention
+// checks too).
+void check_kv4_attention(const Kv4AttentionArgs& a);
+void check_kv4_chunk(const Kv4AttentionArgs& a);
 // Sequences above row_limit, tcgen05 tiles of 128 rows (no lse, no weights).
 size_t kv4_chunk_workspace_bytes(int Hq, int Hkv, int D, size_t n_seq, size_t tokens, int sm_count);
 void launch_kv4_chunk(const Kv4AttentionArgs& a, void* workspace, cudaStream_t s);

@@ -192,12 +192,6 @@ int rs_qwen_kv4_attention(const rs_qwen_kv4_cache* cache, const rs_qwen_kv4_atte
          "kv4 attention: lse and weights must be 4-byte aligned");
     need(args->weights_out || !args->weights_in, "kv4 attention: weights_in needs weights_out");
     need(!args->weights_out || args->weights_stride >= 1, "kv4 attention: weights_stride must be positive");
-    OnDevice on(cache->device);
-    QWEN_CUDA(cudaDeviceGetAttribute(&a.sm_count, cudaDevAttrMultiProcessorCount, cache->device));
-    need(args->workspace && aligned(args->workspace, 16) &&
-             args->workspace_bytes >= kv4_workspace_bytes(cache->q_heads, cache->kv_heads, cache->head_dim, args->n_seq,
-                                                          args->tokens, a.sm_count),
-         "kv4 attention: workspace missing, not 16-byte aligned or smaller than rs_qwen_kv4_workspace_bytes");
     a.q = rows(args->q, args->dtype, "kv4 attention: q must be aligned to its type");
     a.gate = rows(args->gate, RS_QWEN_F32, "kv4 attention: the gate must be 4-byte aligned");
     rows(args->out, args->dtype, "kv4 attention: out must be aligned to its type");
@@ -219,6 +213,13 @@ int rs_qwen_kv4_attention(const rs_qwen_kv4_cache* cache, const rs_qwen_kv4_atte
     a.weights_stride = args->weights_stride;
     a.workspace = args->workspace;
     a.workspace_bytes = args->workspace_bytes;
+    check_kv4_attention(a);
+    OnDevice on(cache->device);
+    QWEN_CUDA(cudaDeviceGetAttribute(&a.sm_count, cudaDevAttrMultiProcessorCount, cache->device));
+    need(args->workspace && aligned(args->workspace, 16) &&
+             args->workspace_bytes >= kv4_workspace_bytes(cache->q_heads, cache->kv_heads, cache->head_dim, args->n_seq,
+                                                          args->tokens, a.sm_count),
+         "kv4 attention: workspace missing, not 16-byte aligned or smaller than rs_qwen_kv4_workspace_bytes");
     launch_kv4_attention(a, static_cast<cudaStream_t>(stream));
   });
 }

@@ -927,6 +927,17 @@ size_t decode_workspace(int Hq, int Hkv, int D, size_t n_seq, size_t tokens, int
 // behind 3840: 262 and 73 us).
 constexpr int kChunkRows = 32;
 
+bool uses_chunks(const Kv4AttentionArgs& a) {
+  return (a.type == kKv4BF16 || a.coarse) && !a.lse && !a.weights_out && int64_t(a.max_count) * (a.cache.Hq / a.cache.Hkv) > kChunkRows;
+}
+// Tiles of the longest sequence that runs here.
+int most_tiles(const Kv4AttentionArgs& a) {
+  const int64_t rows = int64_t(a.max_count) * (a.cache.Hq / a.cache.Hkv);
+  return int((std::min(rows, uses_chunks(a) ? int64_t(kChunkRows) : rows) + kRowsPerTile - 1) / kRowsPerTile);
+}
+// CTAs per (sequence, KV head) of the weights kernel.
+int64_t weight_chunks(const Kv4AttentionArgs& a) { return (a.table_stride + kWtWarps * kWtPages - 1) / (kWtWarps * kWtPages); }
+
 template <int D, class T>
 void attend(const Kv4AttentionArgs& a, cudaStream_t s) {
   static std::atomic<uint64_t> configured{0};
@@ -935,11 +946,9 @@ void attend(const Kv4AttentionArgs& a, cudaStream_t s) {
   });
   Kv4AttentionArgs b = a;
   const int G = a.cache.Hq / a.cache.Hkv, ctas = a.sm_count * kCtasPerSm;
-  const bool chunks = (a.type == kKv4BF16 || a.coarse) && !a.lse && !a.weights_out && a.max_count * int64_t(G) > kChunkRows;
+  const bool chunks = uses_chunks(a);
   b.row_limit = chunks ? kChunkRows : INT_MAX;
-  const int tiles = (int(std::min(int64_t(a.max_count) * G, int64_t(b.row_limit))) + kRowsPerTile - 1) / kRowsPerTile;
-  if (int64_t(a.n_seq) * a.cache.Hkv * tiles > (int64_t(1) << 30) / (a.table_stride / 2 + 1 + kUnitPairs))
-    throw std::invalid_argument("kv4 attention: n_seq x kv_heads x query tiles x pages beyond 2^31; split the call");
+  const int tiles = most_tiles(a);
   const bool q_vec = reinterpret_cast<uintptr_t>(a.q.data) % 16 == 0 && a.q.token_stride % 8 == 0 && a.q.head_stride % 8 == 0;
   const bool gate_vec = reinterpret_cast<uintptr_t>(a.gate.data) % 16 == 0 && a.gate.token_stride % 4 == 0 && a.gate.head_stride % 4 == 0;
   const bool vec = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_token_stride % 8 == 0 && a.out_head_stride % 8 == 0;
@@ -952,9 +961,8 @@ void attend(const Kv4AttentionArgs& a, cudaStream_t s) {
   g_kernel_launches.fetch_add(2, std::memory_order_relaxed);
   if (chunks) launch_kv4_chunk(b, static_cast<uint8_t*>(a.workspace) + decode_workspace(a.cache.Hq, a.cache.Hkv, D, a.n_seq, a.tokens, a.sm_count), s);
   if (a.weights_out) {
-    const int64_t chunks = (a.table_stride + kWtWarps * kWtPages - 1) / (kWtWarps * kWtPages);
-    if (chunks * a.n_seq * a.cache.Hkv > INT32_MAX) throw std::invalid_argument("kv4 attention: n_seq x kv_heads x pages beyond 2^31; split the call");
-    launch_pdl(kv4_weights_kernel<D, T>, unsigned(chunks * a.n_seq * a.cache.Hkv), kWtWarps * 32, 0, s, b, int(chunks), q_vec);
+    const int64_t pieces = weight_chunks(a);
+    launch_pdl(kv4_weights_kernel<D, T>, unsigned(pieces * a.n_seq * a.cache.Hkv), kWtWarps * 32, 0, s, b, int(pieces), q_vec);
     g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
   }
 }
@@ -966,8 +974,17 @@ size_t kv4_workspace_bytes(int Hq, int Hkv, int D, size_t n_seq, size_t tokens, 
          align16(tokens * size_t(Hq) * 4);
 }
 
+void check_kv4_attention(const Kv4AttentionArgs& a) {
+  if (int64_t(a.n_seq) * a.cache.Hkv * most_tiles(a) > (int64_t(1) << 30) / (a.table_stride / 2 + 1 + kUnitPairs))
+    throw std::invalid_argument("kv4 attention: n_seq x kv_heads x query tiles x pages beyond 2^31; split the call");
+  if (uses_chunks(a)) check_kv4_chunk(a);
+  if (a.weights_out && weight_chunks(a) * a.n_seq * a.cache.Hkv > INT32_MAX)
+    throw std::invalid_argument("kv4 attention: n_seq x kv_heads x pages beyond 2^31; split the call");
+}
+
 void launch_kv4_attention(const Kv4AttentionArgs& a, cudaStream_t s) {
   if (a.tokens <= 0 || a.n_seq <= 0) return;
+  check_kv4_attention(a);
   const bool half = a.type == kKv4F16;
   if (a.cache.D == 64) half ? attend<64, __half>(a, s) : attend<64, __nv_bfloat16>(a, s);
   else if (a.cache.D == 128) half ? attend<128, __half>(a, s) : attend<128, __nv_bfloat16>(a, s);

@@ -832,15 +832,16 @@ __global__ void __launch_bounds__(256) kv4_chunk_merge_kernel(Kv4AttentionArgs a
   }
 }
 
+// Tiles of the longest sequence.
+int most_tiles(const Kv4AttentionArgs& a) { return int((int64_t(a.max_count) * (a.cache.Hq / a.cache.Hkv) + kRows - 1) / kRows); }
+
 template <int D, class T>
 void chunk(const Kv4AttentionArgs& a, void* workspace, cudaStream_t s) {
   static std::atomic<uint64_t> configured{0};
   once_per_device(configured, [] {
     QWEN_CUDA(cudaFuncSetAttribute(kv4_chunk_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(Smem<D>))));
   });
-  const int G = a.cache.Hq / a.cache.Hkv, tiles = (a.max_count * G + kRows - 1) / kRows;
-  if (int64_t(a.n_seq) * a.cache.Hkv * tiles > (int64_t(1) << 30) / (a.table_stride / kBlockPages + 1 + kUnitBlocks))
-    throw std::invalid_argument("kv4 attention: n_seq x kv_heads x query tiles x pages beyond 2^31; split the call");
+  const int G = a.cache.Hq / a.cache.Hkv, tiles = most_tiles(a);
   const bool q_vec = reinterpret_cast<uintptr_t>(a.q.data) % 16 == 0 && a.q.token_stride % 8 == 0 && a.q.head_stride % 8 == 0;
   const bool gate_vec = reinterpret_cast<uintptr_t>(a.gate.data) % 16 == 0 && a.gate.token_stride % 4 == 0 && a.gate.head_stride % 4 == 0;
   const bool vec = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_token_stride % 8 == 0 && a.out_head_stride % 8 == 0;
@@ -854,6 +855,11 @@ void chunk(const Kv4AttentionArgs& a, void* workspace, cudaStream_t s) {
 
 size_t kv4_chunk_workspace_bytes(int Hq, int Hkv, int D, size_t n_seq, size_t tokens, int sm_count) {
   return align16(unit_entries(tokens, n_seq, Hq / Hkv, Hkv) * 8) + size_t(sm_count) * 2 * kRows * (D + 2) * 4;
+}
+
+void check_kv4_chunk(const Kv4AttentionArgs& a) {
+  if (int64_t(a.n_seq) * a.cache.Hkv * most_tiles(a) > (int64_t(1) << 30) / (a.table_stride / kBlockPages + 1 + kUnitBlocks))
+    throw std::invalid_argument("kv4 attention: n_seq x kv_heads x query tiles x pages beyond 2^31; split the call");
 }
 
 void launch_kv4_chunk(const Kv4AttentionArgs& a, void* workspace, cudaStream_t s) {

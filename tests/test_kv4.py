@@ -138,3 +138,14 @@ def test_empty_calls_succeed_without_a_device(pkg):
     pkg._call("rs_qwen_kv4_attention", c, C.byref(attention(pkg, n_seq=0)), None)
     pkg._call("rs_qwen_kv4_evict", c, C.byref(evict(pkg, n_seq=0)), None)
     pkg._call("rs_qwen_kv4_read", c, 0, None, 0, None, None, None)
+
+
+@pytest.mark.parametrize("kw", [
+    # 2^20 tiles of 128 rows, each of up to 2^20 blocks of 64 keys
+    dict(dtype=2, n_seq=1, tokens=1 << 26, max_count=1 << 26, table_stride=1 << 22),
+    # with weights: 2^16 tiles of 8 rows over up to 2^23 page pairs, and 2^18 pieces of 64 pages for each of 2^15 sequences
+    dict(n_seq=1 << 15, tokens=1 << 15, max_count=1, table_stride=1 << 24, weights_out=FAKE, weights_stride=1 << 28),
+    dict(n_seq=1 << 12, tokens=1 << 26, max_count=1 << 14, table_stride=1 << 24)])
+def test_attention_refuses_too_much_work_before_any_launch(pkg, kw):
+    """The kernels' 32-bit places: such a call is refused on the host's values alone, with nothing enqueued."""
+    refused(pkg, "rs_qwen_kv4_attention", cache(pkg), attention(pkg, **kw), "split the call")

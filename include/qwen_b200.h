@@ -514,8 +514,12 @@ int rs_qwen_kv4_read(const rs_qwen_kv4_cache* cache, size_t tokens, const int64_
  * which round keys, values and softmax weights to fp16 (2^-11 each). All others
  * use the stored nibbles exactly, with softmax weights to 2^-11 (bf16) or 2^-22
  * (fp16): ask for bf16 where long prefills should be fast. max_count may be
- * larger than any sequence needs, or than `tokens`. A call's n_seq x kv_heads x
- * query tiles x pages must stay below 2^31 (an error otherwise: split the call). */
+ * larger than any sequence needs, or than `tokens`. The kernels count in 32 bits:
+ * a call is accepted while kv_heads x (tokens x G / 8 + n_seq) x (table_stride / 2
+ * + 5) is below 2^30 and n_seq x kv_heads x (max_count x G / 8 + 1) below 2^31, with
+ * G = q_heads / kv_heads, and may be an error beyond (split it). Sequences that
+ * overlap (cu_seqlens not ascending) and exceed that together set the status bit
+ * and give zero rows. */
 typedef struct {
   rs_qwen_kv4_rows q, gate, out;
   uint32_t dtype, reserved;

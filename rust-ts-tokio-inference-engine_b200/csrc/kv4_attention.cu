@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
     int n = 0;
     for (int s = gi * per; s < min(a.n_seq, (gi + 1) * per); ++s) {
       const Seq q = load_seq(a, s, G, blockIdx.x == 0);
-      n += seq_length(q, G) * Hkv;
+      n = add_places(n, seq_length(q, G) * Hkv);
       sm.first[gi] = q.first;
       sm.count[gi] = q.count;
       sm.len[gi] = q.len;
@@ -146,18 +146,23 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+      if (lane >= o) x = add_places(x, y);
     }
     if (lane == 31) sm.scan[warp] = x;
     __syncthreads();
     int before = total;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += sm.scan[w];
-      total += sm.scan[w];
+      if (w < warp) before = add_places(before, sm.scan[w]);
+      total = add_places(total, sm.scan[w]);
     }
     if (gi < groups) sm.offsets[gi] = before + x - n;
     __syncthreads();
+  }
+  const bool over = total == kPlacesMax;
+  if (over) {
+    if (blockIdx.x == 0 && tid == 0) kv4_flag(a.cache.status, kErrBounds);
+    total = 0;
   }
   if (tid == 0) sm.offsets[groups] = total;
   __syncthreads();
@@ -175,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
       for (int s = gi * per; s < min(a.n_seq, (gi + 1) * per); ++s) {
         const Seq q = seq_at(s);
         for (int i = 0; i < Hkv * q.tiles; ++i) {
-          const int n = unit_length(q, i % q.tiles, G), w0 = at / range;
+          const int n = over ? 0 : unit_length(q, i % q.tiles, G), w0 = at / range;
           ws.units[unit_index(q, s, i % q.tiles, i / q.tiles, G, Hkv)] =
               make_int2(w0 * 2 + (at > w0 * range ? 1 : 0), n ? (at + n - 1) / range - w0 + 1 : 0);
           at += n;
@@ -826,7 +831,8 @@ __global__ void __launch_bounds__(kWtWarps * 32) kv4_weights_kernel(Kv4Attention
         const int row = r * kRowsPerTile + t16 / 16, token = row / G;
         const bool real = token < seq.count;
         sm.lse[i][t16 / 16] = real ? a.lse[size_t(seq.first + token) * a.cache.Hq + g * G + row % G] * 1.4426950408889634f : 0.f;
-        if (!real) sm.seen[i][t16 / 16] = 0;
+        // nor does a row without a sum: all its keys are absent, or the call was too large
+        if (!real || sm.lse[i][t16 / 16] == -INFINITY) sm.seen[i][t16 / 16] = 0;
       }
     }
     __syncthreads();
@@ -975,8 +981,10 @@ size_t kv4_workspace_bytes(int Hq, int Hkv, int D, size_t n_seq, size_t tokens, 
 }
 
 void check_kv4_attention(const Kv4AttentionArgs& a) {
-  if (int64_t(a.n_seq) * a.cache.Hkv * most_tiles(a) > (int64_t(1) << 30) / (a.table_stride / 2 + 1 + kUnitPairs))
-    throw std::invalid_argument("kv4 attention: n_seq x kv_heads x query tiles x pages beyond 2^31; split the call");
+  // places of all units (the last pair of an odd table counts whole), and the merge's grid
+  if (tiles_at_most(a, most_tiles(a), kRowsPerTile) * a.cache.Hkv >= kPlacesMax / (a.table_stride / 2 + 1 + kUnitPairs) ||
+      int64_t(a.n_seq) * a.cache.Hkv * most_tiles(a) > INT32_MAX)
+    throw std::invalid_argument("kv4 attention: kv_heads x query tiles x pages beyond 2^31; split the call");
   if (uses_chunks(a)) check_kv4_chunk(a);
   if (a.weights_out && weight_chunks(a) * a.n_seq * a.cache.Hkv > INT32_MAX)
     throw std::invalid_argument("kv4 attention: n_seq x kv_heads x pages beyond 2^31; split the call");

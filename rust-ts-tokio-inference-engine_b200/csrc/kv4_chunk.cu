@@ -227,22 +227,27 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
   for (int g0 = 0; g0 < groups; g0 += kThreads) {
     const int gi = g0 + tid;
     int n = 0;
-    for (int s = gi * per; s < min(a.n_seq, (gi + 1) * per); ++s) n += seq_length(seq_at(s)) * Hkv;
+    for (int s = gi * per; s < min(a.n_seq, (gi + 1) * per); ++s) n = add_places(n, seq_length(seq_at(s)) * Hkv);
     int x = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+      if (lane >= o) x = add_places(x, y);
     }
     if (lane == 31) sm.scan[warp] = x;
     __syncthreads();
     int before = total;
     for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) before += sm.scan[w];
-      total += sm.scan[w];
+      if (w < warp) before = add_places(before, sm.scan[w]);
+      total = add_places(total, sm.scan[w]);
     }
     if (gi < groups) sm.offsets[gi] = before + x - n;
     __syncthreads();
+  }
+  const bool over = total == kPlacesMax;
+  if (over) {
+    if (blockIdx.x == 0 && tid == 0) kv4_flag(a.cache.status, kErrBounds);
+    total = 0;
   }
   if (tid == 0) sm.offsets[groups] = total;
   __syncthreads();
@@ -254,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
       for (int s = gi * per; s < min(a.n_seq, (gi + 1) * per); ++s) {
         const Seq q = seq_at(s);
         for (int i = 0; i < Hkv * q.tiles; ++i) {
-          const int n = unit_length(q, i % q.tiles, G), w0 = at / range;
+          const int n = over ? 0 : unit_length(q, i % q.tiles, G), w0 = at / range;
           ws.units[unit_index(q, s, i % q.tiles, i / q.tiles, G, Hkv)] =
               make_int2(w0 * 2 + (at > w0 * range ? 1 : 0), n ? (at + n - 1) / range - w0 + 1 : 0);
           at += n;
@@ -858,8 +863,9 @@ size_t kv4_chunk_workspace_bytes(int Hq, int Hkv, int D, size_t n_seq, size_t to
 }
 
 void check_kv4_chunk(const Kv4AttentionArgs& a) {
-  if (int64_t(a.n_seq) * a.cache.Hkv * most_tiles(a) > (int64_t(1) << 30) / (a.table_stride / kBlockPages + 1 + kUnitBlocks))
-    throw std::invalid_argument("kv4 attention: n_seq x kv_heads x query tiles x pages beyond 2^31; split the call");
+  if (tiles_at_most(a, most_tiles(a), kRows) * a.cache.Hkv >= kPlacesMax / (a.table_stride / kBlockPages + 1 + kUnitBlocks) ||
+      int64_t(a.n_seq) * a.cache.Hkv * most_tiles(a) > INT32_MAX)
+    throw std::invalid_argument("kv4 attention: kv_heads x query tiles x pages beyond 2^31; split the call");
 }
 
 void launch_kv4_chunk(const Kv4AttentionArgs& a, void* workspace, cudaStream_t s) {

@@ -1,5 +1,6 @@
 // Device helpers shared by the kernels that read the 4-bit KV cache.
 #pragma once
+#include <algorithm>
 #include <cfloat>
 #include <climits>
 
@@ -11,6 +12,18 @@ namespace qwen {
 namespace {
 
 constexpr int kRowsPerTile = 8;  // query rows of an MMA tile
+
+// The attention kernels lay a call's units end to end in places counted in 32
+// bits. The host refuses calls that could need kPlacesMax or more; sequences that
+// overlap (cu_seqlens not ascending) can still exceed what it counted, so the sums
+// stop at kPlacesMax, and a call whose sum reaches it computes nothing.
+constexpr int kPlacesMax = (1 << 30) - 1;
+__device__ __forceinline__ int add_places(int a, int b) { return min(a + b, kPlacesMax); }
+// Tiles of `rows` query rows that a call's sequences fill at most: each the longest's,
+// and together no more than the rows there are, plus a part of a tile each.
+inline int64_t tiles_at_most(const Kv4AttentionArgs& a, int64_t of_longest, int rows) {
+  return std::min(int64_t(a.n_seq) * of_longest, int64_t(a.tokens) * (a.cache.Hq / a.cache.Hkv) / rows + a.n_seq);
+}
 
 // Bounded waits on a barrier; a wait that runs out (about a second) sets the
 // status bit and, where the CTA has roles that wait for one another, `abort`,

@@ -763,3 +763,36 @@ def test_prefill_decode_evict_decode(pkg, heads, rope):
     for counts in ([1, 1], [5, 1], [1, 20], [1, 1]):
         step(counts)
     cache.check()
+
+
+# ------------------------------------------------------------------ the size of a call
+
+def test_a_long_chunk_beside_many_decoding_sequences(pkg):
+    """What bounds a call is the rows and pages that it has, not the longest chunk times the sequences: 129 decoding
+    sequences and 2048 tokens of another, under a table for 262144 tokens, with statistics (8-row tiles) and without."""
+    lens, counts = [1 + (i * 53) % 300 for i in range(129)] + [2100], [1] * 129 + [2048]
+    seqs = Sequences(pkg, lens, (4, 2, 64), seed=41, pad_columns=(1 << 14) - 132)
+    assert seqs.table.shape[1] == 1 << 14
+    q, cu, host = seqs.queries(counts, torch.bfloat16)
+    out, lse, weights = attend(pkg, seqs, q, cu, counts, stats=True)
+    check_attention(seqs, q, host, out, lse, weights)
+    del weights
+    plain, _, _ = attend(pkg, seqs, q, cu, counts)
+    check_attention(seqs, q, host, plain)
+    seqs.cache.check()
+
+
+def test_overlapping_sequences_beyond_the_bound_compute_nothing(pkg):
+    """1201 sequences over the same 4096 rows, 65536 keys each: 1.2e9 places, where the rows there are allow 5e6."""
+    seqs = Sequences(pkg, [16], (1, 1, 64), seed=42)
+    n, T, pages = 2401, 4096, 4096
+    q = torch.randn(T, 1, 64, device="cuda").half()
+    cu = torch.tensor([0, T] * (n // 2 + 1), dtype=torch.int32, device="cuda")
+    lens = torch.full((n,), 16 * pages, dtype=torch.int32, device="cuda")
+    table = seqs.table[0, 0].expand(n, pages).contiguous()
+    out, lse = torch.full_like(q, 77.0), torch.full((T, 1), 77.0, device="cuda")
+    ws = torch.empty(seqs.cache.workspace_bytes(n, T), dtype=torch.uint8, device="cuda")
+    seqs.cache.attention(q, cu, lens, table, out, ws, T, lse=lse)
+    with pytest.raises(pkg.NativeError, match="flag 2"):
+        seqs.cache.check()
+    assert (out == 0).all() and (lse == -math.inf).all()

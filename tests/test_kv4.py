@@ -149,3 +149,14 @@ def test_empty_calls_succeed_without_a_device(pkg):
 def test_attention_refuses_too_much_work_before_any_launch(pkg, kw):
     """The kernels' 32-bit places: such a call is refused on the host's values alone, with nothing enqueued."""
     refused(pkg, "rs_qwen_kv4_attention", cache(pkg), attention(pkg, **kw), "split the call")
+
+
+@pytest.mark.parametrize("stats", [False, True])
+def test_attention_accepts_a_long_chunk_beside_many_sequences(pkg, stats):
+    """The bound counts the rows that a call has, not the longest chunk for every sequence: this one is refused for
+    its missing workspace (or device) alone."""
+    kw = dict(weights_out=FAKE, weights_stride=1 << 18) if stats else {}
+    args = attention(pkg, dtype=2, n_seq=130, tokens=2177, max_count=2048, table_stride=1 << 14, workspace=None, **kw)
+    with pytest.raises(pkg.NativeError) as e:
+        pkg._call("rs_qwen_kv4_attention", C.byref(cache(pkg)), C.byref(args), None)
+    assert "split the call" not in str(e.value)

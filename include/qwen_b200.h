@@ -343,7 +343,10 @@ int rs_qwen_device_synthetic_state(void* session, size_t position, uint64_t seed
  * that the key has received so far (kv_heads x context x 4 bytes per layer and
  * slot, taken from the byte budget), which rs_qwen_device_kv4_evict ranks by; a
  * tracked session refuses mtp_verify_accept, whose rejected tokens would count,
- * and its long prefills run the kernel that keeps softmax statistics. */
+ * and its long prefills run the kernel that keeps softmax statistics, which takes
+ * about nine times as long. A step beyond what the attention kernel counts in 32
+ * bits (rs_qwen_kv4_attention, with table_stride = context / 16) is refused with
+ * its parents as they were. */
 int rs_qwen_device_kv4(void* session, int track, char* error, size_t capacity);
 /* For each of n_seq versions a new version at the same position that holds only
  * `keep` keys per layer and KV head (all, if it has no more): the last `recent`

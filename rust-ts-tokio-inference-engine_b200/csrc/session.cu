@@ -601,6 +601,22 @@ struct Session {
   // Row of slot 0 in one layer's accumulated weights.
   float* kv4_layer_weights(int layer) const { return kv4_weights.p + size_t(layer) * slots * d.Hkv * d.ctx; }
 
+  // The attention call of a step of n sequences and T tokens, as far as its size goes.
+  Kv4AttentionArgs kv4_call(int layer, int n, int T) const {
+    Kv4AttentionArgs t;
+    t.cache = kv4_view(layer);
+    t.n_seq = n;
+    t.tokens = T;
+    t.max_count = kv4_max_count;
+    t.table_stride = bt_stride;
+    t.coarse = true;  // fp16 rows on the 128-row tiles: as the other fp16 operands of the projections
+    if (kv4_track) {
+      t.weights_in = t.weights_out = kv4_layer_weights(layer);
+      t.weights_stride = d.ctx;
+    }
+    return t;
+  }
+
   // Norm, rotation, 4-bit append and attention of one layer's projection: fp16
   // queries (|q| is bounded by the norm: sqrt(head_dim) times its gain) and rows out.
   void kv4_attention(const LayerDev& ly, int proj_w, int splits, size_t split_stride, int n, int T, cudaStream_t s) {
@@ -625,25 +641,17 @@ struct Session {
     a.gate_out = gate.p;
     launch_kv4_append(a, s);
     const int64_t row = int64_t(d.Hq) * d.D;
-    Kv4AttentionArgs t;
-    t.cache = a.cache;
+    Kv4AttentionArgs t = kv4_call(ly.type_index, n, T);
     t.q = {q.p, row, d.D};
     t.gate = {gate.p, row, d.D};
     t.out = hb2.p;
     t.out_token_stride = row;
     t.out_head_stride = d.D;
-    t.n_seq = n;
-    t.tokens = T;
-    t.max_count = kv4_max_count;
     t.cu_seqlens = cu_seqlens.p;
     t.kv_lens = kv4_lens.p;
     t.table = kv4_table.p;
-    t.table_stride = bt_stride;
     t.scale = 1.f / std::sqrt(float(d.D));
-    t.coarse = true;  // as the other fp16 operands of the projections
     if (kv4_track) {
-      t.weights_in = t.weights_out = kv4_layer_weights(ly.type_index);
-      t.weights_stride = d.ctx;
       t.weights_in_rows = kv4_parents.p;
       t.weights_out_rows = kv4_children.p;
     }
@@ -914,6 +922,7 @@ struct Session {
       if (vin && kv4_track) throw std::invalid_argument("speculative verify on a session that tracks attention weights");
       kv4_max_count = 0;
       for (const auto& s : seqs) kv4_max_count = std::max(kv4_max_count, int(s.count));
+      check_kv4_attention(kv4_call(0, n, T));  // before a parent is released
     } else if (d.n_attn > 0) {
       const int G = d.Hq / d.Hkv;
       const bool pf_ok = G >= 1 && G <= 16 && 16 % G == 0;

@@ -411,3 +411,54 @@ def test_more_pages_in_the_same_budget(pkg, make):
         with pytest.raises(pkg.NativeError, match="budget|exhausted"):
             sess.synthetic_state(CONTEXT, 9)
         sess.close()
+
+
+@pytest.mark.gpu
+def test_a_long_prompt_beside_many_decoding_sequences(pkg, store):
+    """A tracked session with room for 262144 tokens: 129 sequences decode while one feeds 2048 tokens. Caches are
+    those of the same tokens fed apart, to a 4-bit step, and every row gives a weight of one to each KV head's keys."""
+    n, ctx, long = 129, 1 << 18, 2048
+    s = pkg.DeviceSession(store, tiny(pkg, ctx), 2 * n + 4, 3 << 30).kv4(track=True)
+    parents, _, _ = s.step_ragged([None] * n, [0] * n, [5] * n, prompt(5 * n, 11))
+    tails, text = prompt(n, 12), prompt(long, 13)
+    alone = []
+    for i in (0, 64, n - 1):
+        (c,), _, _ = s.step_ragged([parents[i]], [5], [1], tails[i:i + 1])
+        alone.append((i, s.kv4_read(c, 0)))
+        s.release(c)
+    (c,), _, _ = s.step_ragged([None], [0], [long], text)
+    alone.append((n, s.kv4_read(c, 0)))
+    s.release(c)
+    kids, _, _ = s.step_ragged(parents + [None], [5] * n + [0], [1] * n + [long], np.concatenate([tails, text]),
+                               flags=pkg.RAGGED_SAMPLED | pkg.RAGGED_CONSUME)
+    for i, held in alone:
+        fed = long if i == n else 6
+        k, v, w = s.kv4_read(kids[i], 0, weights=True)
+        for a, b in zip(held[:2], (k, v)):
+            a, b = np.float64(a), np.float64(b)
+            assert a.shape == b.shape == (KV_HEADS, fed, DIM)
+            # projections of another batch size may be summed in another order: a nibble moves by one at most, scale
+            # and bias by a bf16 step (2^-7 of themselves)
+            low, high = a.min(-1, keepdims=True), a.max(-1, keepdims=True)
+            tol = (high - low) * (1 / 15 + 2.0 ** -7) + 2.0 ** -7 * np.maximum(abs(low), abs(high))
+            assert (abs(a - b) <= tol).all()
+        # beside the rows' own weight, each key's sum of at most G * fed terms is rounded to 32 bits
+        assert (abs(w.sum(1, dtype=np.float64) - G * fed) <= (WEIGHT_TOL + G * fed * 2.0 ** -24) * G * fed).all()
+    assert s.drain() == n + 1
+    s.close()
+
+
+@pytest.mark.gpu
+def test_a_step_that_is_too_large_keeps_its_parents(pkg, store):
+    """2049 tokens over a table of 2^21 pages pass the places that the attention kernel counts in 32 bits: the step is
+    refused before the parent that it would consume is released."""
+    s = pkg.DeviceSession(store, tiny(pkg, 1 << 25), 3, 2 << 30).kv4(track=True)
+    (a,), _, _ = s.step_ragged([None], [0], [3], prompt(3))
+    before = s.kv4_read(a, 0, weights=True)
+    with pytest.raises(pkg.NativeError, match="split the call"):
+        s.step_ragged([a], [3], [2049], prompt(2049, 2), flags=pkg.RAGGED_SAMPLED | pkg.RAGGED_CONSUME)
+    assert all(np.array_equal(x, y) for x, y in zip(before, s.kv4_read(a, 0, weights=True)))
+    (b,), _, _ = s.step_ragged([a], [3], [100], prompt(100, 3), flags=pkg.RAGGED_SAMPLED | pkg.RAGGED_CONSUME)
+    assert s.kv4_read(b, 0)[0].shape[1] == 103
+    assert s.drain() == 1
+    s.close()

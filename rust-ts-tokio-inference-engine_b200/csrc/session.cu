@@ -512,8 +512,10 @@ struct Session {
     // KV page pool: what the byte budget leaves after the DeltaNet pool,
     // capped by free device memory (keep 2 GiB of headroom).
     page_bytes = size_t(d.n_attn) * 2 * d.Hkv * kPageTokens * d.D * 2;
-    size_t budget_pages = 0;
     const uint64_t fixed = uint64_t(n_slots) * gdn_slot_bytes;
+    kv.Hkv = d.Hkv;
+    kv.D = d.D;
+    size_t budget_pages = 0;
     if (d.n_attn > 0) {
       if (bytes <= fixed) throw std::invalid_argument("state byte budget smaller than the DeltaNet pool");
       budget_pages = (bytes - fixed) / page_bytes;
@@ -523,15 +525,17 @@ struct Session {
       size_t mem_pages = free_b > headroom ? (free_b - headroom) / page_bytes : 0;
       budget_pages = std::min({budget_pages, mem_pages, size_t(INT32_MAX / kPageTokens)});
       if (budget_pages == 0) throw std::runtime_error("no device memory left for KV pages");
-      kv_mem.ensure(budget_pages * (page_bytes / 2));
     }
+    make_bf16_pool(budget_pages);
+  }
+
+  void make_bf16_pool(size_t pages) {
+    if (pages) kv_mem.ensure(pages * (page_bytes / 2));
     kv.base = kv_mem.p;
-    kv.n_pages = int(budget_pages);
+    kv.n_pages = int(pages);
     kv.layers = d.n_attn;
-    kv.Hkv = d.Hkv;
-    kv.D = d.D;
-    for (int l = 0; l < d.n_attn && budget_pages > 0; ++l) kv_maps.push_back(make_kv_map(kv, l));
-    reset_pages(budget_pages);
+    for (int l = 0; l < d.n_attn && pages > 0; ++l) kv_maps.push_back(make_kv_map(kv, l));
+    reset_pages(pages);
   }
 
   void reset_pages(size_t n) {
@@ -542,7 +546,8 @@ struct Session {
   }
 
   // ------------------------------------------------------------ 4-bit pages --
-  // rs_qwen_device_kv4: the page pool in 4 bits, in the same byte budget.
+  // rs_qwen_device_kv4: the page pool in 4 bits, in the same byte budget. On an error
+  // the session is as it was, on bf16 pages.
   void kv4_enable(bool track) {
     if (kv4_on) throw std::invalid_argument("4-bit pages already in use");
     if (d.n_attn == 0) throw std::invalid_argument("4-bit pages need an attention layer");
@@ -557,33 +562,41 @@ struct Session {
       throw std::invalid_argument("state byte budget smaller than the DeltaNet pool and the tracked weights");
     set_device();
     QWEN_CUDA(cudaStreamSynchronize(stream));
+    const size_t headroom = size_t(2) << 30, bf16_pages = size_t(kv.n_pages), bf16_page = page_bytes;
+    size_t free_b = 0, total_b = 0;
+    QWEN_CUDA(cudaMemGetInfo(&free_b, &total_b));
+    // what the device can give: its free memory and the bf16 pool, less the headroom and the weights
+    const uint64_t there = uint64_t(free_b) + kv_mem.n * sizeof(*kv_mem.p), taken = headroom + uint64_t(slots) * weight_elems * 4;
+    const size_t pages = std::min({size_t((limit - fixed) / layers_page), there > taken ? size_t((there - taken) / layers_page) : size_t(0),
+                                   size_t(INT32_MAX / kPageTokens)});
+    if (pages == 0) throw std::runtime_error("no device memory left for KV pages");
     reset_pages(0);
     kv_maps.clear();
     kv_mem.release();
     kv.base = nullptr;
     kv.layers = kv.n_pages = 0;
+    try {
+      if (track) kv4_weights.ensure(weight_elems * slots);
+      kv4_mem.ensure(pages * layers_page);
+      kv4_lens.ensure(max_seqs);
+      kv4_new_lens.ensure(max_seqs);
+      kv4_parents.ensure(max_seqs);
+      kv4_children.ensure(max_seqs);
+      kv4_dropped.ensure(max_seqs);
+      kv4_slots.ensure(max_tokens);
+    } catch (...) {  // another program may have taken memory in the meantime
+      kv4_weights.release();
+      kv4_mem.release();
+      cudaGetLastError();
+      page_bytes = bf16_page;
+      make_bf16_pool(bf16_pages);
+      throw;
+    }
     kv4_on = true;
+    kv4_track = track;
     kv4_page = page;
     page_bytes = layers_page;
-    if (track) {
-      kv4_weights.ensure(weight_elems * slots);
-      kv4_weight_bytes = weight_elems * 4;
-      kv4_track = true;
-    }
-    size_t free_b = 0, total_b = 0;
-    QWEN_CUDA(cudaMemGetInfo(&free_b, &total_b));
-    const size_t headroom = size_t(2) << 30;
-    const size_t pages = std::min({size_t((limit - fixed) / page_bytes),
-                                   free_b > headroom ? (free_b - headroom) / page_bytes : size_t(0),
-                                   size_t(INT32_MAX / kPageTokens)});
-    if (pages == 0) throw std::runtime_error("no device memory left for KV pages");
-    kv4_mem.ensure(pages * page_bytes);
-    kv4_lens.ensure(max_seqs);
-    kv4_new_lens.ensure(max_seqs);
-    kv4_parents.ensure(max_seqs);
-    kv4_children.ensure(max_seqs);
-    kv4_dropped.ensure(max_seqs);
-    kv4_slots.ensure(max_tokens);
+    kv4_weight_bytes = weight_elems * 4;
     kv.n_pages = int(pages);
     reset_pages(pages);
   }

@@ -462,3 +462,23 @@ def test_a_step_that_is_too_large_keeps_its_parents(pkg, store):
     assert s.kv4_read(b, 0)[0].shape[1] == 103
     assert s.drain() == 1
     s.close()
+
+
+@pytest.mark.gpu
+def test_a_session_that_cannot_track_keeps_its_pages(pkg, store):
+    """Weights of 6000 slots of 2^22 tokens (201 GB) fit the byte budget and not the device: refused, and the session
+    goes on with bf16 pages, or with 4-bit pages that do not track."""
+    s = pkg.DeviceSession(store, tiny(pkg, 1 << 22), 6000, 1 << 38)
+    with pytest.raises(pkg.NativeError, match="no device memory"):
+        s.kv4(track=True)
+    toks = prompt(20)
+    (a,), first, _ = s.step_ragged([None], [0], [20], toks)
+    with pytest.raises(pkg.NativeError, match="not 4-bit"):
+        s.kv4_read(a, 0)
+    s.release(a)
+    s.kv4()
+    (a,), _, _ = s.step_ragged([None], [0], [20], toks)
+    k, v, _ = s.kv4_read(a, 0)
+    assert k.shape == (KV_HEADS, 20, DIM) and np.isfinite(k).all() and np.isfinite(v).all() and k.any() and v.any()
+    assert s.drain() == 1
+    s.close()

@@ -335,7 +335,8 @@ int rs_qwen_device_synthetic_state(void* session, size_t position, uint64_t seed
  * values in 4 bits (the groups, rounding and layout of the rs_qwen_kv4 section
  * below) instead of bf16: 3.56 times the pages in the same byte budget, and as
  * much less to read per step. Call it before any admission and before
- * mtp_attach; the MTP draft head keeps bf16 pages. Steps, blocks, verify, forks,
+ * mtp_attach; the MTP draft head keeps bf16 pages, one for each page of this pool
+ * (at most slots x context), beside the byte budget. Steps, blocks, verify, forks,
  * synthetic states and snapshots then work on the 4-bit pages (a snapshot holds
  * the values as read back). head_dim must be 64, 128 or 256 with at most 16 query
  * heads per KV head.

@@ -1544,9 +1544,11 @@ struct Session {
     if (mtp_on) throw std::invalid_argument("MTP already attached");
     if (table->residents()) throw std::invalid_argument("MTP attach must precede admission");
     mpage_bytes = size_t(2) * d.Hkv * kPageTokens * d.D * 2;
-    // as many pages as the target pool (one attention layer each), at least a
-    // full context for every slot when the target has no attention layers
-    size_t pages = d.n_attn > 0 ? size_t(kv.n_pages) : slots * size_t(bt_stride);
+    // as many pages as the target pool (one attention layer each), and no more
+    // than a full context for every slot: a 4-bit target pool holds 3.56 times the
+    // pages of a bf16 one, which drafts of short contexts could not fill
+    const size_t all_slots = slots * size_t(bt_stride);
+    size_t pages = d.n_attn > 0 ? std::min(size_t(kv.n_pages), all_slots) : all_slots;
     size_t free_b = 0, total_b = 0;
     QWEN_CUDA(cudaMemGetInfo(&free_b, &total_b));
     const size_t headroom = size_t(2) << 30;

@@ -482,3 +482,17 @@ def test_a_session_that_cannot_track_keeps_its_pages(pkg, store):
     assert k.shape == (KV_HEADS, 20, DIM) and np.isfinite(k).all() and np.isfinite(v).all() and k.any() and v.any()
     assert s.drain() == 1
     s.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv4", [False, True])
+def test_draft_pool_holds_no_more_than_the_slots_can(pkg, make, store, kv4):
+    """The draft head's bf16 pages: a context for each of 24 slots (6.3 MB), not one for every page of the target's
+    pool (256 MB in bf16, 955 MB beside 4-bit pages)."""
+    s = make(kv4)
+    free = torch.cuda.mem_get_info()[0]
+    s.mtp_attach(store)
+    # beside it block tables, hidden rows and weights' scratch: a few MB, in allocations of 2 MB granularity
+    assert free - torch.cuda.mem_get_info()[0] <= 32 << 20
+    (a,), _, _ = s.step_ragged([None], [0], [40], prompt(40), flags=pkg.RAGGED_SAMPLED)
+    s.release(a)

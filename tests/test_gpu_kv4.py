@@ -796,3 +796,36 @@ def test_overlapping_sequences_beyond_the_bound_compute_nothing(pkg):
     with pytest.raises(pkg.NativeError, match="flag 2"):
         seqs.cache.check()
     assert (out == 0).all() and (lse == -math.inf).all()
+
+
+def test_evict_copies_nothing_from_a_page_that_is_not_there(pkg):
+    """Keys of a source page outside the pool are skipped: their places in the destination, every page that is no
+    destination, and the other sequence stay byte for byte what they were."""
+    heads = (4, 2, 64)
+    seqs = Sequences(pkg, [40, 40], heads, seed=43, extra_pages=8)
+    page = pkg.kv4_page_bytes(2, 64)
+    weights = torch.rand(2, 2, seqs.table.shape[1] * 16, generator=seqs.gen, device="cuda")
+    good = seqs.pool.clone()
+    dst, kept, lens, _ = run_evict(pkg, seqs, weights, 24, 4)
+    check_evict(seqs, weights, 24, 4, dst, kept, lens, None)
+    whole = seqs.pool.clone()
+    seqs.pool.copy_(good)
+    seqs.table[0, 1] = 1 << 24
+    dst, again, lens, _ = run_evict(pkg, seqs, weights, 24, 4)
+    with pytest.raises(pkg.NativeError, match="flag 2"):
+        seqs.cache.check()
+    assert torch.equal(again, kept) and lens.tolist() == [24, 24]
+    now, was, full = (x.view(-1, page) for x in (seqs.pool, good, whole))
+    other = torch.ones(now.shape[0], dtype=torch.bool, device="cuda")
+    other[dst.flatten().long()] = False
+    assert torch.equal(now[other], was[other])
+    assert torch.equal(now[dst[1].long()], full[dst[1].long()])
+    p = torch.arange(24, device="cuda")
+    slots = dst[0, p // 16].long() * 16 + p % 16
+    k, v = read(seqs.cache, slots)  # 0xFF bytes read as NaN: the places that were not written
+    for h in range(2):
+        gone = kept[0, h] // 16 == 1
+        assert gone.any() and not gone.all()
+        for got, x in ((k, seqs.k), (v, seqs.v)):
+            assert torch.isnan(got[gone, h]).all()
+            assert torch.equal(got[~gone, h].double(), x[0][kept[0, h].long()[~gone], h])

@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
           tc_fence_before();
           const float2 info = sm.kinfo[n & 7];
           const int absent = __float_as_int(info.y);
-          float fk = fine ? fmaxf(f1 * info.x, FLT_MIN) : NAN;  // above zero: a masked -infinity stays one
+          float fk = fmaxf(f1 * info.x, FLT_MIN);  // above zero: a masked -infinity stays one
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.s_empty);
           const int key0 = j * kKeys + kMine * half;
@@ -757,7 +757,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
           const int e2 = sm.ve[(n - 1) & 7][c / 64];
           float f = pow2i(e2 == kNone ? 0 : e2 / 2) * (whole ? inv : 1.f);
           const float f2 = pow2i(e2 == kNone ? 0 : e2 - e2 / 2);
-          if (poison >> (c / 64) & 1) f = NAN;
+          // a query that is not finite went in as zeros: NaN where the row has seen a key, and zero where it has none
+          if ((poison >> (c / 64) & 1) || (!fine && l != 0.f)) f = NAN;
           if (real) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {

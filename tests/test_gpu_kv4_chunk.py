@@ -39,6 +39,9 @@ def check_rows(seqs, s, q, out, scale=None, hidden=()):
     NaN makes its group of 64 dims NaN in the rows that see it, a key all of them."""
     n, L, G = q.shape[0], seqs.lens[s], seqs.Hq // seqs.Hkv
     scale = scale or seqs.D ** -0.5
+    if not L:
+        assert (out == 0).all()
+        return
     k, v = seqs.k[s].repeat_interleave(G, 1), seqs.v[s].repeat_interleave(G, 1)
     bad_k, bad_v = torch.isnan(k).any(-1), torch.isnan(v)  # [L, Hq], [L, Hq, D]
     j = torch.arange(L, device="cuda")
@@ -55,7 +58,7 @@ def check_rows(seqs, s, q, out, scale=None, hidden=()):
     most = seqs.most[s].nan_to_num().amax(0).repeat_interleave(G, 0)
     mass = torch.einsum("nhd,hd->nh", q.double().nan_to_num(0, 0, 0).abs(), most) * scale
     ds = (2.0 ** -11 + seqs.D * 2.0 ** -23) * mass
-    vmax = v.nan_to_num().abs().max() if L else 0.0
+    vmax = v.nan_to_num().abs().max()
     loose = (3 * 2.0 ** -11 + 2 * ds[..., None] + 2.0 ** -18) * vmax
     tol = 2.0 ** -8 * (ref.abs() + loose) + loose
     d = (out.double() - ref).abs()
@@ -85,6 +88,24 @@ def test_nan_reaches_only_the_rows_that_see_it(pkg, heads):
     for s in range(2):
         check_rows(seqs, s, q[host[s]:host[s + 1]], out[host[s]:host[s + 1]])
     seqs.cache.check()
+
+
+@pytest.mark.parametrize("heads", HEADS + [(6, 6, 64)])
+def test_rows_that_see_no_key(pkg, heads):
+    """More query tokens than cached keys: the first ones are zero, whatever their query row holds; a row with a NaN
+    or an infinity that sees a key is NaN."""
+    lens, counts = [3, 0, 20, 100], [40, 36, 164, 150]
+    seqs = Sequences(pkg, lens, heads, seed=51)
+    q, cu, host = seqs.queries(counts, torch.bfloat16)
+    out = attend(seqs, q, cu, counts)
+    check_attention(seqs, q, host, out)
+    for s, (n, c) in enumerate(zip(lens, counts)):
+        for row, value in ((0, math.nan), (c - n - 1, math.inf), (min(c - 1, c - n + 1), math.nan), (c - 1, math.inf)):
+            q[host[s] + row, row % heads[0], 5] = value
+    out = attend(seqs, q, cu, counts)
+    for s, (n, c) in enumerate(zip(lens, counts)):
+        check_rows(seqs, s, q[host[s]:host[s + 1]], out[host[s]:host[s + 1]])
+        assert (out[host[s]:host[s] + c - n] == 0).all()
 
 
 @pytest.mark.parametrize("spread,scale", [(30.0, 0.0), (1.0, 8.0), (1e-4, 0.25), (3e4, 1e-6), (1e4, 1e4)])

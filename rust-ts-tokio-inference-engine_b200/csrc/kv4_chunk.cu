@@ -99,7 +99,7 @@ struct Smem {
   alignas(16) uint32_t vst[kSets][D / 64][kKeys / 2][4];  // V: the same for the two keys of a pair
   // by block: K's power of two, V's of every group and the one before, the keys
   // (even, odd of each pair) whose group is NaN
-  alignas(8) float2 kinfo[8];               // K's power times 2^-16, and the bits of the pages that are not there
+  alignas(8) float2 kinfo[8];               // K's power times 2^-10, and the bits of the pages that are not there
   alignas(4) uint8_t vflags[8][4];          // by group: 1 the power has moved, 2 it holds a NaN
   int ve[8][D / 64], ve_was[8][D / 64];
   uint32_t vnan[8][D / 64][2];
@@ -163,7 +163,8 @@ struct Power {
   __device__ __forceinline__ void raise(float most, bool first) {
     if (first) *this = Power();
     if (__any_sync(0xffffffffu, most > limit && most < INFINITY)) {
-      const int top = int(__reduce_max_sync(0xffffffffu, most < INFINITY ? __float_as_uint(most) : 0u) >> 23) - 126;
+      // not below -125, so that 2^(e - 10) is a normal number
+      const int top = max(int(__reduce_max_sync(0xffffffffu, most < INFINITY ? __float_as_uint(most) : 0u) >> 23) - 126, -125);
       e = top + 9;
       limit = e > 133 ? FLT_MAX : pow2i(e - 6);
       down = pow2i(-e / 2);
@@ -442,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
           const float s = kv4_scale(own[i]) * power.down * power.down2 * 1048576.f, b = kv4_bias(own[i]) * power.down * power.down2;
           *reinterpret_cast<uint4*>(sm.kst[n % kSets][lane + 32 * i][dw]) = make_uint4(pack_f16(s * 16.f, s * 16.f), pack_f16(s, s), pack_f16(b, b), 0u);
         }
-        if (dt == 0) sm.kinfo[n & 7] = make_float2(power.e == kNone ? 0.f : pow2i(power.e - 16), __int_as_float(sm.absent[n & 7]));
+        if (dt == 0) sm.kinfo[n & 7] = make_float2(power.e == kNone ? 0.f : pow2i(power.e - 10), __int_as_float(sm.absent[n & 7]));
       }
       asm volatile("bar.sync 1, %0;" ::"n"(kDeqWarps * 32) : "memory");
     };
@@ -612,7 +613,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
           for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(kv4_to_float(x[e])) & 0x7FFFFFFFu);
         }
         const bool fine = most < 0x7F800000u;
-        const int e = most && fine ? int(most >> 23) - 126 : 0;
+        // at least -110: f1 below is then a normal number, and fp16 has room for the smaller row
+        const int e = most && fine ? max(int(most >> 23) - 126, -110) : 0;
         const float up = pow2i((14 - e) / 2), up2 = fine ? pow2i(14 - e - (14 - e) / 2) : 0.f;
 #pragma unroll 1
         for (int d = 64 * half; d < D; d += 128) {
@@ -632,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.q_full);
         const float factor = a.scale * 1.4426950408889634f;
-        const float f1 = factor * pow2i((e + 2) / 2) * pow2i(e + 2 - (e + 2) / 2);  // 2^(e - 14), and the 2^16 that K's power lacks
+        const float f1 = factor * pow2i((e - 4) / 2) * pow2i(e - 4 - (e - 4) / 2);  // 2^(e - 14), and the 2^10 that K's power lacks
         const int seen = real ? q.len - q.count + token + 1 : INT_MAX;
         const int least = __reduce_min_sync(0xffffffffu, seen);
         uint32_t poison = 0u;  // groups of which the row sees a NaN

@@ -118,6 +118,17 @@ def test_large_and_small_logits(pkg, heads, spread, scale):
     check_attention(seqs, q, host, out, scale=scale)
 
 
+@pytest.mark.parametrize("key,query", [(1e-36, 1e36), (1e-37, 1e37), (1e-38, 3e37), (1e36, 1e-36), (1e-30, 1.0), (3e37, 1e-37), (3e37, 1e-38)])
+def test_products_of_far_magnitudes(pkg, key, query):
+    """Keys and queries at opposite ends of the range: their product is an ordinary logit."""
+    heads = (8, 1, 128)
+    seqs = Sequences(pkg, [200], heads, seed=53, spread=key)
+    q, cu, host = seqs.queries([60], torch.float32)
+    q = (q * query).to(torch.bfloat16)
+    out = attend(seqs, q, cu, [60])
+    check_rows(seqs, 0, q, out)
+
+
 @pytest.mark.parametrize("heads", HEADS)
 def test_pages_out_of_range_count_as_absent(pkg, heads):
     lens, counts = [40, 300, 33], [36, 290, 33]

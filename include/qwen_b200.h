@@ -434,8 +434,8 @@ int rs_qwen_project_noalloc(void* session, int which, int layer, const void* x_d
  * head) in groups of 64 dims:
  *   scale = bf16((max - min) / 15), bias = bf16(min),
  *   n = clamp(rint((x - bias) / scale), 0, 15), value = scale * n + bias
- * (n = 0 where scale is 0; a group that holds an infinity or NaN reads back as
- * NaN). A page holds 16 tokens; slot = page * 16 + offset. Of each (page, KV
+ * (n = 0 where scale is 0; a group that holds an infinity or NaN, or whose minimum
+ * rounds to an infinity in bf16, reads back as NaN). A page holds 16 tokens; slot = page * 16 + offset. Of each (page, KV
  * head) the pool keeps 18 * head_dim bytes (4.5 bits per value; csrc/kv4.h has
  * the layout), so pool bytes = pages * rs_qwen_kv4_page_bytes.
  *

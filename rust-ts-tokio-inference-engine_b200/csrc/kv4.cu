@@ -79,7 +79,8 @@ __device__ __forceinline__ double higher(double a, double b) { return a > b ? a 
 
 // Quantises a warp's row (lane l holds dims l E .. l E + E - 1; V: 32 or 64 bits)
 // and writes nibbles and pairs of token `tok` of `block`. A group with a value
-// that is not finite gets a NaN bias: every value of it then reads back as NaN.
+// that is not finite, or whose minimum rounds to an infinity in bf16, gets a NaN
+// bias: every value of it then reads back as NaN.
 // A nibble is rint((x - bias) / step), by its exact value: found in 32 bits when
 // that is safely away from the border between two nibbles, and by the division in
 // 64 bits when not (bf16 inputs lie exactly on the border often enough to show).
@@ -103,6 +104,7 @@ __device__ __forceinline__ void quantise_store(const V (&x)[D / 32], uint8_t* bl
     hi = higher(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
   __nv_bfloat16 scale = __float2bfloat16_rn(float((double(hi) - double(lo)) / 15.0)), bias = __float2bfloat16_rn(float(lo));
+  fine = fine && (__bfloat16_as_ushort(bias) & 0x7F80) != 0x7F80;  // a minimum that bf16 has no number for
   if (!fine) {
     scale = __ushort_as_bfloat16(0);
     bias = __ushort_as_bfloat16(0x7FC0);

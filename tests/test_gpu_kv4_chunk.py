@@ -90,6 +90,26 @@ def test_nan_reaches_only_the_rows_that_see_it(pkg, heads):
     seqs.cache.check()
 
 
+@pytest.mark.parametrize("value", [-3.4e38, 3.4e38])
+@pytest.mark.parametrize("stats", [False, True])
+def test_minimum_that_bf16_has_no_number_for(pkg, value, stats):
+    """A finite 32-bit group whose minimum rounds to an infinity in bf16 is stored as NaN, so rows that do not see it
+    are untouched (an infinite operand times a weight of zero would be NaN in all of them)."""
+    seqs = Sequences(pkg, [170], (8, 1, 128), seed=60)
+    q, cu, host = seqs.queries([170], torch.bfloat16)
+    v = torch.randn(1, 1, 128, generator=seqs.gen, device="cuda")
+    v[:, :, 64:] = value
+    zero = torch.zeros_like(v)
+    seqs.cache.append(None, zero, v, None, seqs.slots(0, 69, 70), None)
+    k, got = torch.empty_like(v), torch.empty_like(v)
+    seqs.cache.read(seqs.slots(0, 69, 70), k, got)
+    assert torch.isnan(got[..., 64:]).all() and torch.equal(got[..., :64].double(), quantised(v)[0][..., :64])
+    seqs.k[0][69], seqs.v[0][69], seqs.most[0][69] = 0, got[0].double(), 0
+    lse = torch.empty(170, 8, device="cuda") if stats else None  # with it, the 8-row kernel
+    out = attend(seqs, q, cu, [170], lse=lse)
+    check_rows(seqs, 0, q, out)
+
+
 @pytest.mark.parametrize("heads", HEADS + [(6, 6, 64)])
 def test_rows_that_see_no_key(pkg, heads):
     """More query tokens than cached keys: the first ones are zero, whatever their query row holds; a row with a NaN

@@ -54,11 +54,11 @@ double g_routing_slack = 2e-3;
 int g_emulate = 0;
 
 // Keys and values of the fed tokens that a quantising cache holds, [attention
-// layers][K, V][kv][tokens][d]: attention then reads these, each checked to be
-// within `g_kv_slack` of a 4-bit step of the oracle's own. Null: its own.
+// layers][K, V][kv][tokens][d]: attention then reads these, each checked to be what
+// 4-bit storage can make of the oracle's own, computed to `g_kv_slack`. Null: its own.
 const float* g_forced_kv = nullptr;
 size_t g_forced_kv_layer = 0;
-double g_kv_slack = 5e-2;
+double g_kv_slack = 5e-3;  // of a group's norm; fp16 operands move a logits row by 2.7e-3
 
 double round16(double v) {
   if (g_emulate & 256) return double(float(_Float16(float(v))));
@@ -463,10 +463,14 @@ struct Forward {
             double* own = (sel ? Vc : Kc) + (g * ctx + offset + t) * d;
             const float* held = g_forced_kv + (((g_forced_kv_layer * 2 + sel) * Hk + g) * T + t) * d;
             for (size_t i0 = 0; i0 < d; i0 += 64) {
-              const double range = *std::max_element(own + i0, own + i0 + 64) - *std::min_element(own + i0, own + i0 + 64);
-              // half a step; sqrt 2 of it where a key was rotated after it was stored
+              const double low = *std::min_element(own + i0, own + i0 + 64), high = *std::max_element(own + i0, own + i0 + 64);
+              double norm = 0;
+              for (size_t i = i0; i < i0 + 64; ++i) norm += own[i] * own[i];
+              // half a step of range / 15; the bf16 scale (15 steps of it) and bias, 2^-9 each, in the value and in
+              // what it is clamped to; sqrt 2 of all that where a key was rotated after it was stored
+              const double stored = (high - low) / 30 + std::ldexp(high - low + std::abs(low), -8);
               for (size_t i = i0; i < i0 + 64; ++i) {
-                if (!(std::abs(held[i] - own[i]) <= (std::sqrt(2.) / 30 + g_kv_slack) * range + g_kv_slack * std::abs(own[i])))
+                if (!(std::abs(held[i] - own[i]) <= std::sqrt(2.) * stored + g_kv_slack * std::sqrt(norm)))
                   throw std::invalid_argument("oracle: the cached key or value is not near the oracle's");
                 own[i] = double(held[i]);
               }

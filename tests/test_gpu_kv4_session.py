@@ -496,3 +496,43 @@ def test_draft_pool_holds_no_more_than_the_slots_can(pkg, make, store, kv4):
     assert free - torch.cuda.mem_get_info()[0] <= 32 << 20
     (a,), _, _ = s.step_ragged([None], [0], [40], prompt(40), flags=pkg.RAGGED_SAMPLED)
     s.release(a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("track", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dim,rope", [(4, 2, 128, 32), (6, 1, 64, 64)])
+def test_other_heads_against_the_oracle(pkg, O, heads, kv_heads, dim, rope, track):
+    """A prompt of 700 tokens in one step (several tokens per CTA of the append, split projection sums and gates), a
+    block of 40 (128-row tiles of fp16 rows without tracking) and single tokens."""
+    if not has_cuda():
+        pytest.skip("no CUDA device")
+    O.set_routing_slack(5e-2)
+
+    def config(mod):
+        return mod.config(hidden=256, layers=4, vocab=4096, q_heads=heads, kv_heads=kv_heads, head_dim=dim, key_heads=2,
+                          value_heads=4, key_dim=64, value_dim=64, experts=16, top=2, intermediate=128, shared=128,
+                          context=1024, rope_dims=rope, theta=THETA)
+
+    store = pkg.WeightStore().synthetic(config(pkg), SEED)
+    s = pkg.DeviceSession(store, config(pkg), slots=4, budget_bytes=1 << 28).kv4(track)
+    model = O.Model(config(O), SEED)
+    try:
+        s.set_capture(True)
+        toks = prompt(742, 21)
+        cur, state, pos = None, None, 0
+        for n in (700, 40, 1, 1):
+            (cur,), _, logits = s.step_ragged([cur], [pos], [n], toks[pos:pos + n],
+                                              flags=pkg.RAGGED_LOGITS | pkg.RAGGED_ALL_ROWS)
+            route = s.debug_routing(n)
+            held = np.stack(s.kv4_read(cur, 0)[:2])[None, :, :, pos:]
+            lg, _, _, _ = model.forward(toks[pos:pos + n], pos, old_state=state, forced_routing=route, cached_kv=held)
+            assert max(rel_l2(logits[j], lg[j]) for j in range(n)) <= 1e-2  # the tolerance of the bf16 sessions
+            state, pos = s.snapshot(cur), pos + n
+        if track:
+            w = s.kv4_read(cur, 0, weights=True)[2]
+            g = heads // kv_heads
+            assert (abs(w.sum(1, dtype=np.float64) - g * pos) <= (WEIGHT_TOL * dim / 64 + g * pos * 2.0 ** -24) * g * pos).all()
+        s.release(cur)
+    finally:
+        s.close()
+        store.close()

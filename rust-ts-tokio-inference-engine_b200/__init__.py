@@ -605,6 +605,7 @@ class Kv4Cache:
     def __init__(self, pool, q_heads: int, kv_heads: int, head_dim: int, status=None):
         import torch
         self._current_stream = torch.cuda.current_stream
+        self._synchronize = torch.cuda.synchronize
         self._f32, self._i32, self._i64, self._u8 = torch.float32, torch.int32, torch.int64, torch.uint8
         self._types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
         page = kv4_page_bytes(kv_heads, head_dim)
@@ -736,8 +737,10 @@ class Kv4Cache:
         _call("rs_qwen_kv4_evict", self._ref, C.byref(args), self._stream(stream))
 
     def check(self):
-        """Reads and clears the status word (synchronises); raises if a kernel met an index out of range."""
+        """Reads and clears the status word; raises if a kernel met an index out of range. Waits for the whole device:
+        calls may have been made on any of its streams."""
         if self.status is not None:
+            self._synchronize(self.device)
             bits = int(self.status.item())
             if bits:
                 self.status.zero_()

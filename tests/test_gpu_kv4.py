@@ -829,3 +829,21 @@ def test_evict_copies_nothing_from_a_page_that_is_not_there(pkg):
         for got, x in ((k, seqs.k), (v, seqs.v)):
             assert torch.isnan(got[gone, h]).all()
             assert torch.equal(got[~gone, h].double(), x[0][kept[0, h].long()[~gone], h])
+
+
+def test_check_waits_for_calls_on_other_streams(pkg):
+    """An index out of range that a call on another stream is still to meet."""
+    cache = new_cache(pkg, (2, 1, 64), 2)
+    x, slots = torch.randn(1, 1, 64, device="cuda"), torch.tensor([1 << 20], device="cuda")
+    a = torch.randn(8192, 8192, device="cuda")
+    b = torch.mm(a, a)
+    cache.append(None, x, x, None, slots % 32, None)  # kernels are loaded, which can wait for the device
+    cache.check()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(10):
+            torch.mm(a, a, out=b)
+    cache.append(None, x, x, None, slots, None, stream=side)
+    with pytest.raises(pkg.NativeError, match="flag 2"):
+        cache.check()
+    cache.check()  # cleared

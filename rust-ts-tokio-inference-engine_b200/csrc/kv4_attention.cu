@@ -180,9 +180,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
       for (int s = gi * per; s < min(a.n_seq, (gi + 1) * per); ++s) {
         const Seq q = seq_at(s);
         for (int i = 0; i < Hkv * q.tiles; ++i) {
-          const int n = over ? 0 : unit_length(q, i % q.tiles, G), w0 = at / range;
+          const int n = unit_length(q, i % q.tiles, G), w0 = at / range;
           ws.units[unit_index(q, s, i % q.tiles, i / q.tiles, G, Hkv)] =
-              make_int2(w0 * 2 + (at > w0 * range ? 1 : 0), n ? (at + n - 1) / range - w0 + 1 : 0);
+              make_int2(w0 * 2 + (at > w0 * range ? 1 : 0), n && !over ? (at + n - 1) / range - w0 + 1 : 0);
           at += n;
         }
       }
@@ -830,9 +830,10 @@ __global__ void __launch_bounds__(kWtWarps * 32) kv4_weights_kernel(Kv4Attention
       if (t16 % 16 == 0) {
         const int row = r * kRowsPerTile + t16 / 16, token = row / G;
         const bool real = token < seq.count;
-        sm.lse[i][t16 / 16] = real ? a.lse[size_t(seq.first + token) * a.cache.Hq + g * G + row % G] * 1.4426950408889634f : 0.f;
-        // nor does a row without a sum: all its keys are absent, or the call was too large
-        if (!real || sm.lse[i][t16 / 16] == -INFINITY) sm.seen[i][t16 / 16] = 0;
+        // a row without a sum (all its keys are absent, or the call was too large) gives no weight: exp(x - infinity)
+        const float lse = real ? a.lse[size_t(seq.first + token) * a.cache.Hq + g * G + row % G] * 1.4426950408889634f : 0.f;
+        sm.lse[i][t16 / 16] = lse == -INFINITY ? INFINITY : lse;
+        if (!real) sm.seen[i][t16 / 16] = 0;
       }
     }
     __syncthreads();

@@ -260,9 +260,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
       for (int s = gi * per; s < min(a.n_seq, (gi + 1) * per); ++s) {
         const Seq q = seq_at(s);
         for (int i = 0; i < Hkv * q.tiles; ++i) {
-          const int n = over ? 0 : unit_length(q, i % q.tiles, G), w0 = at / range;
+          const int n = unit_length(q, i % q.tiles, G), w0 = at / range;
           ws.units[unit_index(q, s, i % q.tiles, i / q.tiles, G, Hkv)] =
-              make_int2(w0 * 2 + (at > w0 * range ? 1 : 0), n ? (at + n - 1) / range - w0 + 1 : 0);
+              make_int2(w0 * 2 + (at > w0 * range ? 1 : 0), n && !over ? (at + n - 1) / range - w0 + 1 : 0);
           at += n;
         }
       }

@@ -344,8 +344,10 @@ int rs_qwen_device_synthetic_state(void* session, size_t position, uint64_t seed
  * that the key has received so far (kv_heads x context x 4 bytes per layer and
  * slot, taken from the byte budget), which rs_qwen_device_kv4_evict ranks by; a
  * tracked session refuses mtp_verify_accept, whose rejected tokens would count,
- * and its long prefills run the kernel that keeps softmax statistics, which takes
- * about nine times as long. A step beyond what the attention kernel counts in 32
+ * and its long prefills run the kernel that keeps softmax statistics (2048 tokens
+ * behind 14336: 15 ms per attention layer instead of 0.75). Without tracking,
+ * sequences that feed more than 32 query rows per KV head run on the 128-row tiles
+ * of rs_qwen_kv4_attention, with their fp16 rounding. A step beyond what the attention kernel counts in 32
  * bits (rs_qwen_kv4_attention, with table_stride = context / 16) is refused with
  * its parents as they were. */
 int rs_qwen_device_kv4(void* session, int track, char* error, size_t capacity);
@@ -517,7 +519,9 @@ int rs_qwen_kv4_read(const rs_qwen_kv4_cache* cache, size_t tokens, const int64_
  * 32 query rows per KV head (max_count x q_heads / kv_heads) run on larger tiles,
  * which round keys, values and softmax weights to fp16 (2^-11 each). All others
  * use the stored nibbles exactly, with softmax weights to 2^-11 (bf16) or 2^-22
- * (fp16): ask for bf16 where long prefills should be fast. max_count may be
+ * (fp16): ask for bf16 where long prefills should be fast. A query row whose
+ * largest magnitude is below 2^-110 keeps fewer bits, and from 2^116 / scale on it
+ * may come out NaN, as with an infinity or NaN in it where it sees a key. max_count may be
  * larger than any sequence needs, or than `tokens`. The kernels count in 32 bits:
  * a call is accepted while kv_heads x (tokens x G / 8 + n_seq) x (table_stride / 2
  * + 5) is below 2^30 and n_seq x kv_heads x (max_count x G / 8 + 1) below 2^31, with

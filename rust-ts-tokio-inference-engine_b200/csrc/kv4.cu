@@ -181,8 +181,10 @@ struct Frequencies {
 // nibbles is then decided by its value, not by the order of a sum, so the same
 // tokens give the same cache whatever the batch around them.
 // 2168 fp32 tokens of 16 + 2 + 2 rows of 256: 28 us (74 MB, 2.6 TB/s; all keys in
-// 64 bits with a division each took 106), bound by the instructions of the key rows;
-// 64 bf16 tokens: 6.5 us (11), the latency of one sine and one row.
+// 64 bits with a division each took 106). Neither bytes nor one pipe bounds it: issue
+// slots 48 %, warps 40 %, waits for shuffles and 64-bit results first (3.9 cycles an
+// instruction), for memory next (2.7). 64 bf16 tokens: 6.5 us (11), the latency of
+// one sine and one row.
 constexpr int kMaxBatch = 8;
 // kFused: fp32 rows as split-K partials, and a gate beside every query row
 // (the session's projection).
@@ -297,7 +299,8 @@ __global__ void __launch_bounds__(kQ == 1 ? 640 : 256, kQ == 1 ? 1 : 4) kv4_appe
 
 // One thread per 16 bytes of K and of V values of a cached token, so that a warp's
 // stores are contiguous. 121925 tokens of 2 x 256 in fp32 (570 MB): 121 us,
-// 4.7 TB/s (142 us with four items per thread).
+// 4.7 TB/s (142 us with four items per thread); fp16 or bf16 (320 MB): 72 us. Issue
+// slots 62 %, ALU 58 %: the wait for slot, then nibbles, and the unpacking around it.
 template <int D, class T, class Index>
 __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4View c, Index tokens, const int64_t* __restrict__ slots,
                                                        T* k, T* v) {
@@ -347,8 +350,9 @@ constexpr int kSelKeys = 32;  // keys a thread keeps in registers
 // A thread holds consecutive keys, so one prefix sum then gives every kept key its
 // place; keys beyond the first 32 of a thread (more than 32768 in all) are read
 // again in every pass. 64 rows of up to 32768 keys: 39 us (histogram: 66), bound by
-// the compares that the longest row's one SM issues; 16 rows of up to 500: 9.5 us
-// (26), the 32 barriers.
+// the compares that the longest row's one SM issues (issue slots 68 %, ALU 63 % while
+// it runs; the others are long done); 16 rows of up to 500: 9.5 us (26), the 32
+// barriers.
 template <int kKeys>
 __device__ __forceinline__ void select_keys(const float* w, int32_t* kept, float* wo, int n, int m, int per, int (*counts)[kSelThreads / 32]);
 
@@ -480,7 +484,8 @@ __device__ __forceinline__ void select_keys(const float* w, int32_t* kept, float
 // Kept keys to their new places: 16 bytes (4 or 8 for the pairs of narrow heads) a
 // piece, kMovePieces per thread so that their chains of loads (kept index, page
 // ids, bytes) run side by side: 64 rows of 4096 keys (76 MB both ways) in 39 us, 53
-// with one piece per thread. Sources are scattered 32-byte sectors.
+// with one piece per thread. Sources are scattered 32-byte sectors: 64 MB come from
+// memory for the 19 MB of half those rows.
 constexpr int kMovePieces = 4;
 template <int D>
 __global__ void __launch_bounds__(256) kv4_move_kernel(Kv4EvictArgs a, int row_blocks) {

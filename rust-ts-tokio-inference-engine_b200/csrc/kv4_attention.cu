@@ -6,10 +6,11 @@
 // partial results that kv4_merge_kernel joins. The lengths live on the device,
 // so every CTA finds the ranges itself from a prefix sum over the sequences;
 // after it the warps never wait for one another.
-// 64 sequences of 128 to 32768 keys, 2 KV heads of 256 (219 MB): 65 us with
-// the merge behind it, against 33 at the copy's rate. The stream itself runs at the HBM rate; the rest is the
-// start of the ranges, some 14 thousand cycles. 128 sequences of 4 tokens: 100 us,
-// bound by the instructions of the four tiles.
+// 64 sequences of 128 to 32768 keys, 2 KV heads of 256 (219 MB): 66 us with
+// the merge behind it, against 33 at the copy's rate. Two things fill the rest: an
+// SM has work for 105 of the profiled launch's 135 thousand cycles, for equal
+// ranges do not end together, and some 14 thousand of them start the ranges. 128
+// sequences of 4 tokens: 100 us, bound by the instructions of the four tiles.
 //
 // A warp streams its pages through a private shared-memory ring, one bulk copy
 // per (page, KV head) block, across unit borders, and works on 2 x 16 keys x 8
@@ -23,7 +24,9 @@
 //   (0, sum of q), the sums split into three bf16 terms, two MMAs give the
 //   bias part of all 16 keys.
 //   Q is fp16, each row scaled by a power of two, so fp16 and bf16 queries are
-//   exact (bf16 has fewer mantissa bits and the row keeps its range).
+//   exact (bf16 has fewer mantissa bits and the row keeps its range). Brought back,
+//   a row of 2^116 / scale and above overflows and comes out NaN; below 2^-110 the
+//   three terms of its sums lose bits.
 //   O^T += V^T P^T. The nibbles of two keys are interleaved into k pairs and
 //   masked the same way. The step of V is folded into the weights, P_g = p
 //   scale_g, rounded to fp16 (2^-11 of a weight, the operand's own precision)
@@ -623,7 +626,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv4_decode_kernel(Kv4Att
 // Joins the partial results of a unit whose pages span several warps, and writes
 // the rows of a unit that has no page. One CTA per (unit, row): its threads
 // weigh the parts while they fetch them, D / 4 threads to a part. 7 us for 128 units
-// of 8 rows (64 sequences), 16 for 1024: the latency of unit, statistics, parts.
+// of 8 rows (64 sequences), 16 for 1024: the latency of unit, statistics, parts
+// (issue slots 39 %, waits for memory first). The grid has the longest sequence's
+// tiles for every sequence, so many short ones beside a long chunk pay for CTAs that
+// find no row.
 constexpr int kMergeThreads = 128, kMergeFetch = 8;
 template <int D, class T>
 __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(Kv4AttentionArgs a, int workers, int tiles) {
@@ -711,11 +717,14 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(Kv4AttentionAr
 
 // What every cached key received from the call's query rows, added to what it
 // had: sum over the rows of exp(logit - lse), with the logits multiplied again from
-// the exact nibbles, as in the decode kernel (the K half of the pages is read once
-// more; keeping all logits would take 4 bytes per key and query head). One CTA per
+// the exact nibbles, as in the decode kernel. The K half of the pages is read once
+// more, 144 bytes a key at head_dim 256; logits kept in 32 bits would be written and
+// read instead, 8 bytes a key and row, which is less up to 17 rows. One CTA per
 // (sequence, KV head, 64 pages), eight pages per warp; a key's sum belongs to one
 // warp, rows in order, so there are no atomics. 32 sequences of 256 to 16384 keys, 2
-// KV heads of 256: 19 us (2 TB/s of nibbles and weights: latency, not bytes).
+// KV heads of 256: 19 us (2 TB/s of nibbles and weights; issue slots 34 %, waits for
+// memory first: latency, not bytes). 2048 tokens behind 14336 keys: 8.6 ms, the
+// instructions of 2048 tiles.
 constexpr int kWtWarps = 8, kWtPages = 8, kWtTiles = 4;  // pages of a warp; tiles of query rows held at a time
 
 // The query rows of a tile as B fragments (lane = 4 row + t, register j of word
@@ -930,7 +939,7 @@ size_t decode_workspace(int Hq, int Hkv, int D, size_t n_seq, size_t tokens, int
 // of 256), 155 and 184, 191 and 186 (4 of 128). Only bf16 rows go there: its fp16
 // operands (keys, values, weights) leave 3.5e-4 of error, nothing beside bf16's own
 // rounding (1.7e-3) and twice fp16's (2.1e-4). That precision has its price: 2048
-// fp16 tokens behind 14336 keys take 6.2 ms here, bf16 ones 0.71 ms there (256
+// fp16 tokens behind 14336 keys take 6.3 ms here, bf16 ones 0.75 ms there (256
 // behind 3840: 262 and 73 us).
 constexpr int kChunkRows = 32;
 

@@ -12,9 +12,12 @@
 //         each other their maximum, so both hold the row's; sums in registers
 //   8-11  dequantisation of K, 12-15 of V: nibbles -> fp16 operands in the 128B-swizzled layout
 //   16    MMA issue    17, 18  bulk copies of the pages' K and V parts
-// 2048 tokens of 16 + 2 heads of 256 behind 14336 keys: 710 us (0.73 PFLOP/s; 778
-// with one softmax thread per row). What is left is the chain of a block in the
-// dequantisation warps: steps, meeting, values.
+// 2048 tokens of 16 + 2 heads of 256 behind 14336 keys: 750 us a call with its
+// merge (0.69 PFLOP/s; 838 with one softmax thread per row), this kernel alone 731
+// under the profiler. What is left is the chain of a block in the dequantisation
+// warps (steps, meeting, values) and, in the last CTA, the table of the units'
+// parts, which one thread per sequence writes before its range (20 us for 256 units
+// when that loop had one select more).
 // The nibbles of the page layout come out as the operands' element pairs: two
 // dims of a K row, two keys of a V^T row. Masked, a pair is an fp16 subnormal
 // pair n 2^-24 (or n 2^-20), so one fused multiply-add with the step times 2^24
@@ -800,8 +803,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(Kv4AttentionArgs
 }
 
 // Joins the parts of a unit that spans CTAs and writes the rows of one that sees
-// no key. A warp per row, eight rows per CTA: 28 us for 256 units of 128 rows, most of
-// which find nothing to join.
+// no key. A warp per row, eight rows per CTA: 28 us for 256 units of 128 rows, about
+// 150 of which lie in two CTAs (58 MB read; issue slots 37 %, waits for memory
+// first). The grid has the longest sequence's tiles for every sequence: beside 120
+// decoding sequences the same chunk's grid has 496 thousand CTAs, 4096 of them with
+// rows, and the call takes 1.38 ms instead of 0.8.
 template <int D, class T>
 __global__ void __launch_bounds__(256) kv4_chunk_merge_kernel(Kv4AttentionArgs a, void* workspace, int ctas, int tiles) {
   pdl_trigger();

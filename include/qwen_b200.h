@@ -347,9 +347,10 @@ int rs_qwen_device_synthetic_state(void* session, size_t position, uint64_t seed
  * and its long prefills run the kernel that keeps softmax statistics (2048 tokens
  * behind 14336: 15 ms per attention layer instead of 0.75). Without tracking,
  * sequences that feed more than 32 query rows per KV head run on the 128-row tiles
- * of rs_qwen_kv4_attention, with their fp16 rounding. A step beyond what the attention kernel counts in 32
- * bits (rs_qwen_kv4_attention, with table_stride = context / 16) is refused with
- * its parents as they were. */
+ * of rs_qwen_kv4_attention, with their fp16 rounding. A step beyond what the
+ * attention kernel counts in 32 bits (rs_qwen_kv4_attention, with table_stride =
+ * context / 16) is refused with its parents as they were. An error leaves the
+ * session on bf16 pages. */
 int rs_qwen_device_kv4(void* session, int track, char* error, size_t capacity);
 /* For each of n_seq versions a new version at the same position that holds only
  * `keep` keys per layer and KV head (all, if it has no more): the last `recent`

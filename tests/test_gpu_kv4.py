@@ -847,3 +847,66 @@ def test_check_waits_for_calls_on_other_streams(pkg):
     with pytest.raises(pkg.NativeError, match="flag 2"):
         cache.check()
     cache.check()  # cleared
+
+
+def test_weights_and_eviction_captured_and_replayed(pkg):
+    """A graph of attention that accumulates weights in place (the log-sum-exp in the workspace) and of the eviction
+    that ranks by them, against the same calls made one by one, over three replays."""
+    def state():
+        seqs = Sequences(pkg, [100, 37, 300], (16, 2, 256), seed=44, extra_pages=12)
+        q, cu, _ = seqs.queries([1, 2, 40], torch.bfloat16)
+        s = dict(seqs=seqs, q=q, cu=cu, out=torch.zeros_like(q), kept=torch.full((3, 2, 60), -9, dtype=torch.int32, device="cuda"),
+                 lens=torch.zeros(3, dtype=torch.int32, device="cuda"), wo=torch.zeros(3, 2, 64, device="cuda"),
+                 w=torch.rand(3, 2, seqs.table.shape[1] * 16, generator=seqs.gen, device="cuda"),
+                 ws=torch.empty(seqs.cache.workspace_bytes(3, 43), dtype=torch.uint8, device="cuda"),
+                 dst=torch.tensor(seqs.spare[:12], dtype=torch.int32, device="cuda").view(3, 4))
+        return s
+
+    def calls(s):
+        c, k = s["seqs"].cache, s["seqs"]
+        c.attention(s["q"], s["cu"], k.kv_lens, k.table, s["out"], s["ws"], 40, weights_in=s["w"], weights_out=s["w"])
+        c.evict(k.kv_lens, k.table, s["dst"], s["w"], 60, 8, s["kept"], s["lens"], s["wo"])
+
+    one, two = state(), state()
+    torch.cuda.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        calls(one)
+    for _ in range(3):
+        graph.replay()
+        calls(two)
+    torch.cuda.synchronize()
+    for name in ("out", "kept", "lens", "wo", "w"):
+        assert torch.equal(one[name], two[name]), name
+    assert torch.equal(one["seqs"].pool, two["seqs"].pool)
+    want = [U.evicted(two["w"][s, h], n, 60, 8) for s, n in enumerate(two["seqs"].lens) for h in range(2)]
+    got = [[i for i in row if i >= 0] for row in two["kept"].view(6, 60).tolist()]
+    assert got == want
+
+
+def test_calls_from_two_threads(pkg):
+    """Two host threads, each with its own cache, workspace and stream, give what they give one after the other."""
+    import threading
+
+    work = []
+    for i, kind in enumerate((torch.float16, torch.bfloat16)):
+        seqs = Sequences(pkg, [700, 64, 9], (16, 2, 256) if i else (20, 4, 128), seed=45 + i)
+        counts = [60, 1, 3]
+        q, cu, host = seqs.queries(counts, kind)
+        want, _, _ = attend(pkg, seqs, q, cu, counts)
+        work.append([seqs, q, cu, counts, want, torch.cuda.Stream(), []])
+    torch.cuda.synchronize()
+
+    def run(seqs, q, cu, counts, want, stream, got):
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got.append(attend(pkg, seqs, q, cu, counts)[0])
+
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for *_, want, _, got in work:
+        assert len(got) == 20 and all(torch.equal(x, want) for x in got)
